@@ -37,6 +37,9 @@ enum wdg_status {
     WDG_ERR_HIP = -3       /* a HIP runtime call failed: see wdg_last_error */
 };
 
+/* Element types of the entry points that take more than fp32 (layer normalisation, AdamW). */
+enum wdg_type { WDG_F32 = 0, WDG_BF16 = 1, WDG_F16 = 2 };
+
 /* Human-readable text of the last failure on the calling thread. */
 const char* wdg_last_error(void);
 /* Library version / target string, e.g. "wdgan 0.1 gfx950". */
@@ -392,6 +395,25 @@ int wdg_ln_fwd(const float* y, int ldy, const float* gamma, const float* beta, f
 int wdg_ln_bwd(const float* dz, int lddz, const float* y, int ldy, const float* mean_rstd,
                const float* gamma, float act_slope, float* dpre, int lddpre,
                float* dgamma, float* dbeta, float* dbias, int64_t P, int C, wdg_stream stream);
+
+/* LayerNormalization over the last axis of [P][C] rows of any width (1 <= C <= 2^24) in fp32, bf16 or fp16 (wdg_type), forward and
+ * backward (csrc/layernorm.hip) — for the tensors that wdg_ln_fwd / wdg_ln_bwd refuse (16-bit types, C % 4 != 0, C > 1024, odd row
+ * strides), with parameter gradients summed in a fixed order: the same bits on every run.
+ *   - x, z, dz, dx: unit channel stride, row strides in elements, aligned to their element only; input rows may coincide
+ *     (stride 0 = broadcast); z may be x, and dx may be dz or x, element for element; no other overlap;
+ *   - gamma, beta: [C], fp32 or the activations' type (param_type); NULL = ones / zeros;
+ *   - mean_rstd: fp32 [P][2] (mean, 1 / sqrt(var + eps)), written by the forward (NULL: not kept), read by the backward;
+ *   - statistics and sums are fp32; z and dx are rounded once.  A NaN or an infinity makes its own row what the formula makes of it,
+ *     and its column of the parameter gradients.
+ *   - dgamma, dbeta: fp32 [C], either may be NULL; accumulate != 0 adds to them, 0 overwrites them (with zeros when P == 0).
+ *     ws: wdg_layernorm_bwd_ws_bytes() of scratch, needed with either (16-byte aligned, not shared with work that may run at the
+ *     same time). */
+int wdg_layernorm_fwd(const void* x, int64_t ldx, const void* gamma, const void* beta, float eps, void* z, int64_t ldz,
+                      float* mean_rstd, int64_t P, int64_t C, int type, int param_type, wdg_stream stream);
+size_t wdg_layernorm_bwd_ws_bytes(int64_t P, int64_t C, int type);
+int wdg_layernorm_bwd(const void* dz, int64_t lddz, const void* x, int64_t ldx, const float* mean_rstd, const void* gamma, void* dx,
+                      int64_t lddx, float* dgamma, float* dbeta, int accumulate, int64_t P, int64_t C, int type, int param_type,
+                      void* ws, size_t ws_bytes, wdg_stream stream);
 
 /* ------------------------------------------------------------------------------------------
  * ConvLSTM2D cell pointwise part, Keras gate order i,f,c,o, hard_sigmoid = clip(0.2x+0.5,0,1).

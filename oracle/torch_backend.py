@@ -436,6 +436,30 @@ class TorchOps:
             dbias += d.sum(0)
         dpre.copy_(d)
 
+    def layernorm_fwd(self, x, gamma, beta, eps, z, mean_rstd=None):
+        """Any width and type: the 64-bit definition, rounded to the tensors' types on store."""
+        x64 = x.double()
+        mean = x64.mean(1, keepdim=True)
+        rstd = 1.0 / torch.sqrt(((x64 - mean) ** 2).mean(1, keepdim=True) + eps)
+        out = (x64 - mean) * rstd
+        if gamma is not None:
+            out = out * gamma.double()
+        if beta is not None:
+            out = out + beta.double()
+        z.copy_(out)
+        if mean_rstd is not None:
+            mean_rstd.copy_(torch.cat([mean, rstd], 1))
+
+    def layernorm_bwd(self, dz, x, mean_rstd, gamma, dx, dgamma=None, dbeta=None, accumulate=True):
+        g, mr = dz.double(), mean_rstd.double()
+        xh = (x.double() - mr[:, :1]) * mr[:, 1:]
+        a = g if gamma is None else g * gamma.double()
+        d = mr[:, 1:] * (a - a.mean(1, keepdim=True) - xh * (a * xh).mean(1, keepdim=True))
+        for out, total in ((dgamma, (g * xh).sum(0)), (dbeta, g.sum(0))):
+            if out is not None:
+                out.copy_(out.double() + total if accumulate else total)
+        dx.copy_(d)
+
     # ---- ConvLSTM cell: Keras gate order i,f,c,o; hard_sigmoid = clip(.2x+.5,0,1) ------------
     @staticmethod
     def _hs(x):

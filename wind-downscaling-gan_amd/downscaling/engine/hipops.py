@@ -1002,6 +1002,108 @@ class HipOps:
                                          ldd, _ptr(dgamma), _ptr(dbeta), _ptr(dbias), dz.shape[0], dz.shape[1],
                                          self.stream), "ln_bwd")
 
+    # ---- layer norm, any width and type (csrc/layernorm.hip) ---------------------------------------------
+    TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}       # wdg_type
+
+    def _on_device(self, *tensors):
+        for t in tensors:
+            if t is not None and t.device != self.device:
+                raise ValueError(f"tensor on {t.device}, this backend runs on {self.device}")
+
+    @staticmethod
+    def _overlap(a, b):
+        """Whether two tensors may share memory: the address ranges they span meet, and they are not two sets of columns of one buffer."""
+        if a is None or b is None or not a.numel() or not b.numel():
+            return False
+        pa, pb, es = a.data_ptr(), b.data_ptr(), a.element_size()
+        end = lambda t, p: p + t.element_size() * (1 + sum((n - 1) * abs(st) for n, st in zip(t.shape, t.stride())))      # noqa: E731
+        if pa >= end(b, pb) or pb >= end(a, pa):
+            return False
+        if a.dim() == b.dim() == 2 and es == b.element_size() and a.stride() == b.stride() and a.stride(1) == 1 and (pb - pa) % es == 0:
+            ld = a.stride(0)
+            off = ((pb - pa) // es) % ld if ld > 0 else 0
+            return not (off >= a.shape[1] and off + b.shape[1] <= ld)
+        return True
+
+    def _ln_rows(self, name, t, like=None, out=False):
+        """(ptr, row stride) of a [P, C] tensor of layernorm_fwd / _bwd; `out`: rows are written, so they may not overlap."""
+        if t.dim() != 2 or t.dtype not in self.TYPES:
+            raise ValueError(f"{name}: a [P, C] tensor of {', '.join(str(d) for d in self.TYPES)} is wanted, got {t.dtype} {tuple(t.shape)}")
+        if like is not None and (t.shape != like.shape or t.dtype != like.dtype):
+            raise ValueError(f"{name}: {t.dtype} {tuple(t.shape)}, but {like.dtype} {tuple(like.shape)} goes with it")
+        P, Cn = t.shape
+        if Cn < 1 or (Cn > 1 and t.stride(1) != 1) or (out and P > 1 and t.stride(0) < Cn):
+            raise ValueError(f"{name}: shape {tuple(t.shape)}, strides {t.stride()}: channels have to be adjacent" + (" and rows apart" if out else ""))
+        return t.data_ptr(), t.stride(0) if P > 1 else Cn
+
+    def _ln_vec(self, name, v, Cn, dtypes):
+        if v is not None and (v.dtype not in dtypes or tuple(v.shape) != (Cn,) or not v.is_contiguous()):
+            raise ValueError(f"{name}: a contiguous [{Cn}] vector of {' or '.join(str(d) for d in dtypes)} is wanted, got {v.dtype} {tuple(v.shape)}")
+        return v
+
+    def _ln_params(self, x, gamma, beta=None):
+        """wdg_type of the parameters: fp32 or the activations' (both the same)."""
+        for name, v in (("gamma", gamma), ("beta", beta)):
+            self._ln_vec(name, v, x.shape[1], (torch.float32, x.dtype))
+        kinds = {v.dtype for v in (gamma, beta) if v is not None}
+        if len(kinds) > 1:
+            raise ValueError("gamma and beta have to be of one type")
+        return self.TYPES[kinds.pop()] if kinds else 0
+
+    def _ln_stats(self, mean_rstd, P):
+        if mean_rstd is not None and (mean_rstd.dtype != torch.float32 or tuple(mean_rstd.shape) != (P, 2) or not mean_rstd.is_contiguous()):
+            raise ValueError(f"mean_rstd: a contiguous fp32 [{P}, 2] tensor is wanted, got {mean_rstd.dtype} {tuple(mean_rstd.shape)}")
+        return _ptr(mean_rstd)
+
+    def _ln_apart(self, out_name, out, **others):
+        """`out` is written: it may be one of `others` element for element, and meets none of them otherwise."""
+        for name, t in others.items():
+            same = t is not None and t.data_ptr() == out.data_ptr() and t.shape == out.shape and t.stride() == out.stride() and t.dtype == out.dtype
+            if not same and self._overlap(out, t):
+                raise ValueError(f"{out_name} overlaps {name}")
+
+    def layernorm_fwd(self, x, gamma, beta, eps, z, mean_rstd=None):
+        """z = (x - mean) / sqrt(var + eps) * gamma + beta over the last axis of x [P, C], C >= 1 any width, x and z fp32, bf16 or
+        fp16 with adjacent channels and any row stride (wdg_layernorm_fwd).  gamma, beta: [C], fp32 or x's type, or None; mean_rstd:
+        fp32 [P, 2], kept for layernorm_bwd, or None.  z may be x."""
+        self._on_device(x, gamma, beta, z, mean_rstd)
+        px, ldx = self._ln_rows("x", x)
+        pz, ldz = self._ln_rows("z", z, like=x, out=True)
+        kind = self._ln_params(x, gamma, beta)
+        stats = self._ln_stats(mean_rstd, x.shape[0])
+        self._ln_apart("z", z, x=x, gamma=gamma, beta=beta)
+        if mean_rstd is not None:
+            self._ln_apart("mean_rstd", mean_rstd, x=x, z=z, gamma=gamma, beta=beta)
+        with torch.cuda.device(self.device):
+            native.check(self.lib.wdg_layernorm_fwd(px, ldx, _ptr(gamma), _ptr(beta), float(eps), pz, ldz, stats, x.shape[0], x.shape[1],
+                                                    self.TYPES[x.dtype], kind, self.stream), "layernorm_fwd")
+
+    def layernorm_bwd(self, dz, x, mean_rstd, gamma, dx, dgamma=None, dbeta=None, accumulate=True):
+        """Gradients of layernorm_fwd: dx (may be dz or x), and dgamma / dbeta (fp32 [C], added to unless accumulate is False;
+        None: not formed), summed over the rows in a fixed order (wdg_layernorm_bwd)."""
+        self._on_device(dz, x, mean_rstd, gamma, dx, dgamma, dbeta)
+        px, ldx = self._ln_rows("x", x)
+        pg, ldg = self._ln_rows("dz", dz, like=x)
+        pd, ldd = self._ln_rows("dx", dx, like=x, out=True)
+        P, Cn = x.shape
+        kind = self._ln_params(x, gamma)
+        if mean_rstd is None:
+            raise ValueError("mean_rstd of the forward pass is needed")
+        stats = self._ln_stats(mean_rstd, P)
+        self._ln_apart("dx", dx, x=x, dz=dz, mean_rstd=mean_rstd, gamma=gamma)
+        for name, v in (("dgamma", dgamma), ("dbeta", dbeta)):
+            if self._ln_vec(name, v, Cn, (torch.float32,)) is not None:
+                if any(self._overlap(v, o) for o in (x, dz, dx, mean_rstd, gamma)):
+                    raise ValueError(f"{name} overlaps another argument")
+        if self._overlap(dgamma, dbeta):
+            raise ValueError("dgamma overlaps dbeta")
+        with torch.cuda.device(self.device):
+            # scratch of this call alone: the allocator orders its reuse on this stream, and inside a graph capture it belongs to the graph
+            need = int(self.lib.wdg_layernorm_bwd_ws_bytes(P, Cn, self.TYPES[x.dtype])) if dgamma is not None or dbeta is not None else 0
+            ws = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
+            native.check(self.lib.wdg_layernorm_bwd(pg, ldg, px, ldx, stats, _ptr(gamma), pd, ldd, _ptr(dgamma), _ptr(dbeta), int(bool(accumulate)),
+                                                    P, Cn, self.TYPES[x.dtype], kind, _ptr(ws), need, self.stream), "layernorm_bwd")
+
     # ---- ConvLSTM cell ----------------------------------------------------------------------
     def lstm_fwd(self, gates, c_prev, c, h, F):
         pg, ldg = _v2(gates)

@@ -103,6 +103,9 @@ SIGNATURES = {
                                 c_fp, c_fp, c_fp, i64, i32, c_fp]),
     "wdg_ln_fwd": (i32, [c_fp, i32, c_fp, c_fp, f32, c_fp, i32, c_fp, i64, i32, c_fp]),
     "wdg_ln_bwd": (i32, [c_fp, i32, c_fp, i32, c_fp, c_fp, f32, c_fp, i32, c_fp, c_fp, c_fp, i64, i32, c_fp]),
+    "wdg_layernorm_fwd": (i32, [c_fp, i64, c_fp, c_fp, f32, c_fp, i64, c_fp, i64, i64, i32, i32, c_fp]),
+    "wdg_layernorm_bwd_ws_bytes": (szt, [i64, i64, i32]),
+    "wdg_layernorm_bwd": (i32, [c_fp, i64, c_fp, i64, c_fp, c_fp, c_fp, i64, c_fp, c_fp, i32, i64, i64, i32, i32, c_fp, szt, c_fp]),
     "wdg_lstm_fwd": (i32, [c_fp, i32, c_fp, i32, c_fp, i32, c_fp, i32, i64, i32, c_fp]),
     "wdg_lstm_bwd": (i32, [c_fp, i32, c_fp, i32, c_fp, i32, c_fp, i32, c_fp, i32, c_fp, i32, c_fp, i32,
                             i64, i32, c_fp]),
