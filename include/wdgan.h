@@ -710,6 +710,59 @@ int wdg_philox_uniform(float* out, int64_t n, uint64_t seed, uint64_t offset, wd
  * ------------------------------------------------------------------------------------------ */
 int wdg_adam_tf(float* p, const float* g, float* m, float* v, int64_t n, float lr_t, float beta1,
                 float beta2, float eps, float grad_scale, wdg_stream stream);
+
+/* ------------------------------------------------------------------------------------------
+ * AdamW over a list of tensors in one launch (csrc/adamw.hip): decoupled weight decay, states in 32 or 8 bits, gradients optionally
+ * clipped by their global norm.  For every element, with s = grad_scale and t = step (1, 2, ...):
+ *   norm = s sqrt(sum over all tensors of g^2);  c = max_norm > 0 ? max_norm / max(norm, max_norm) : 1;  g' = c s g
+ *   m = beta1 m + (1 - beta1) g';  v = beta2 v + (1 - beta2) g'^2
+ *   p = p (1 - lr weight_decay decay) - lr / (1 - beta1^t) m / (sqrt(v / (1 - beta2^t)) + eps);  copy = p rounded to its type
+ * Arithmetic is fp32 (the norm's sum fp64) whatever the tensors' types; p is rounded once.  With max_norm > 0 a norm that is not
+ * finite leaves weights, copies and states as they were.  Without it a NaN or an infinity goes where the formula takes it.
+ *
+ * 8-bit states: every 256 consecutive elements of a tensor (the last block may be shorter) share two fp32 scales, M = max |m| and
+ * V = max v, and hold   m = M q |q| / 127^2, q = -127 .. 127 (int8),   v = V (q / 255)^4, q = 0 .. 255 (uint8),
+ * q rounded to nearest on the companded value and, for v > 0, at least 1: the second moment of an element that has one never reads as
+ * zero.  Scales below 2^-126 count as zero.  A block that a value which is not finite reaches is NaN from then on.
+ *
+ * Tensors: p, g, copy and fp32 states are aligned to their element; 8-bit states to 4 bytes, and their code arrays span whole blocks of
+ * 256 bytes (codes behind the last element are written as zero).  n == 0 is allowed.  No written range may meet another one or a
+ * gradient: create refuses.  decay: factor of weight_decay for this tensor (0: not decayed).
+ * ------------------------------------------------------------------------------------------ */
+typedef struct wdg_adamw_tensor {
+    void* p;                  /* weights, updated in place */
+    const void* g;            /* gradient */
+    void* m;                  /* first moment: float [n], or int8 codes */
+    void* v;                  /* second moment: float [n], or uint8 codes */
+    float* m_scale;           /* [ceil(n / 256)], 8-bit states only */
+    float* v_scale;
+    void* copy;               /* the updated weights in a second, 16-bit type; or NULL */
+    int64_t n;
+    int32_t p_type, g_type, copy_type;   /* wdg_type */
+    float decay;
+} wdg_adamw_tensor;
+typedef struct wdg_adamw_args {
+    double lr, beta1, beta2, eps, weight_decay, grad_scale, max_norm;   /* max_norm <= 0: no clipping */
+    int64_t step;             /* t, when step_dev is NULL */
+    const int64_t* step_dev;  /* t in device memory (captured steps), read by the launch */
+    float* norm;              /* receives the norm when max_norm > 0, or NULL */
+} wdg_adamw_args;
+typedef struct wdg_adamw_batch wdg_adamw_batch;
+/* Checks the list and lays out its table on the host (no device call); bind copies the table into wdg_adamw_table_bytes() of device
+ * memory that the caller owns and keeps for as long as the batch, or a graph that captured its steps, is used.  bind waits for the
+ * copy: not on the launch path, not while capturing. */
+int wdg_adamw_create(wdg_adamw_batch** out, const wdg_adamw_tensor* tensors, int n, int state_bits /* 32 or 8 */);
+size_t wdg_adamw_table_bytes(const wdg_adamw_batch* b);
+int wdg_adamw_bind(wdg_adamw_batch* b, void* table, size_t table_bytes, wdg_stream stream);
+int wdg_adamw_destroy(wdg_adamw_batch* b);
+/* Scratch of wdg_adamw_step with max_norm > 0 and of wdg_adamw_grad_norm (8-byte aligned, one per call that may run at the same time). */
+size_t wdg_adamw_scratch_bytes(void);
+int wdg_adamw_step(const wdg_adamw_batch* b, const wdg_adamw_args* args, void* scratch, size_t scratch_bytes, wdg_stream stream);
+/* norm[0] = grad_scale sqrt(sum g^2) over all gradients of the batch (0 for none). */
+int wdg_adamw_grad_norm(const wdg_adamw_batch* b, double grad_scale, float* norm, void* scratch, size_t scratch_bytes, wdg_stream stream);
+/* The values that 8-bit states stand for: m_out / v_out [blocks * 256] of type out_type (either may be NULL). */
+int wdg_adamw_moments(const void* m, const float* m_scale, const void* v, const float* v_scale, int64_t blocks, void* m_out, void* v_out,
+                      int out_type, wdg_stream stream);
 /* Zero 1..16 element ranges [begin, end) of a flat fp32 buffer in one launch (begin_end: host array of n pairs, every value a
  * multiple of 4): what `optimizer.zero_grad` leaves of the gradient buffer when the big kernel gradients are stored by their first
  * weight-gradient launch instead of being zero-filled (ganbase.py:39,50: a fresh tape per update). */

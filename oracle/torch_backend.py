@@ -686,3 +686,77 @@ class TorchOps:
         m += (1 - beta1) * (gg - m)
         v += (1 - beta2) * (gg * gg - v)
         p -= lr_t * m / (torch.sqrt(v) + eps)
+
+    def make_adamw(self, entries, state_bits=32, state=None):
+        """Restatement of HipOps.make_adamw in 64 bits, tensor by tensor, block of 256 by block of 256."""
+        ops = self
+
+        class _Batch:
+            def __init__(self):
+                self.entries, self.state_bits = [tuple(e) + (None,) * (4 - len(e)) for e in entries], state_bits
+                self.offsets, self.total = [], 0
+                for p, *_ in self.entries:
+                    self.offsets.append(self.total)
+                    self.total += -(-p.numel() // 256) * 256
+                n = self.total
+                kinds = [(torch.float64, n)] * 2 if state_bits == 32 else [(torch.int8, n), (torch.uint8, n), (torch.float64, n // 256), (torch.float64, n // 256)]
+                self.state = list(state) if state is not None else [torch.zeros(k, dtype=d) for d, k in kinds]
+                self.m, self.v = self.state[:2]
+                self.m_scale, self.v_scale = self.state[2:] if state_bits == 8 else (None, None)
+
+            def values(self):
+                if state_bits == 32:
+                    return self.m.double(), self.v.double()
+                qm, qv = self.m.double(), self.v.double()
+                return (qm * qm.abs() / 127.0 ** 2 * self.m_scale.double().repeat_interleave(256),
+                        (qv / 255.0) ** 4 * self.v_scale.double().repeat_interleave(256))
+
+            def moments(self, m_out=None, v_out=None):
+                for t, s in zip((m_out, v_out), self.values()):
+                    if t is not None:
+                        t.copy_(s)
+
+            def grad_norm(self, norm, grad_scale=1.0):
+                norm.fill_(grad_scale * math.sqrt(sum(float((g.double() ** 2).sum()) for _, g, _, _ in self.entries)))
+
+            @staticmethod
+            def encode(x, second):
+                x = x.view(-1, 256)
+                top = x.abs().amax(1, keepdim=True)
+                top = torch.where(x.isfinite().all(1, keepdim=True), top, torch.full_like(top, float("nan")))
+                top = torch.where(top < 2.0 ** -126, torch.zeros_like(top), top)
+                part = torch.where((top > 0) & x.isfinite(), x.abs() / top, torch.zeros_like(x))
+                if second:
+                    q = torch.where(part > 0, torch.round(255 * part ** 0.25).clamp(min=1), part)
+                    return q.to(torch.uint8).view(-1), top[:, 0]
+                return (torch.round(127 * part.sqrt()) * x.nan_to_num().sign()).to(torch.int8).view(-1), top[:, 0]
+
+            def step(self, t, lr, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=0.0, grad_scale=1.0, max_norm=None, norm=None):
+                t, c = int(t), 1.0
+                if max_norm is not None:
+                    n = torch.zeros(1, dtype=torch.float64)
+                    self.grad_norm(n, grad_scale)
+                    if norm is not None:
+                        norm.copy_(n)
+                    if not math.isfinite(float(n)):
+                        return
+                    c = max_norm / max(float(n), max_norm)
+                ms, vs = self.values()
+                for (p, g, decay, copy), o in zip(self.entries, self.offsets):
+                    k = p.numel()
+                    gg = g.double().view(-1) * (grad_scale * c)
+                    ms[o:o + k] = beta1 * ms[o:o + k] + (1 - beta1) * gg
+                    vs[o:o + k] = beta2 * vs[o:o + k] + (1 - beta2) * gg * gg
+                    upd = ms[o:o + k] / (1 - beta1 ** t) / (torch.sqrt(vs[o:o + k] / (1 - beta2 ** t)) + eps)
+                    new = p.double().view(-1) * (1 - lr * weight_decay * decay) - lr * upd
+                    p.view(-1).copy_(new)
+                    if copy is not None:
+                        copy.view(-1).copy_(new)
+                if state_bits == 32:
+                    self.m.copy_(ms)
+                    self.v.copy_(vs)
+                elif self.total:
+                    for code, scale, (q, top) in ((self.m, self.m_scale, self.encode(ms, False)), (self.v, self.v_scale, self.encode(vs, True))):
+                        code.copy_(q)
+                        scale.copy_(top)
+        return _Batch()

@@ -1,0 +1,489 @@
+// adamw.hip — AdamW over a list of tensors in one launch, states in 32 or 8 bits, with the global gradient norm that clips it.
+// The formulas and the 8-bit format stand at wdg_adamw_step in wdgan.h.
+//
+// The list is cut into chunks of 4096 elements that never cross a tensor; a workgroup takes one chunk and finds everything about it in
+// one record of the table (pointers already advanced), so that no search and no second dependent read stands before the data.
+// A wave takes 256 consecutive elements at a time — four per lane —, which is one block of the 8-bit states: its two maxima are wave
+// maxima and no other wave needs them.
+#include "vec.h"
+#include <algorithm>
+#include <exception>
+#include <math.h>
+#include <vector>
+
+constexpr int AW_CHUNK = 4096;     // elements per record
+constexpr int AW_BLOCK = 256;      // elements that share a scale of the 8-bit states
+constexpr int AW_PARTS = 256;      // partial sums of the gradient norm
+
+struct WdgAdamwChunk {
+    void* p;
+    const void* g;
+    void* m;
+    void* v;
+    float* ms;
+    float* vs;
+    void* copy;
+    int n;                                        // elements, 1 .. AW_CHUNK
+    unsigned char p_type, g_type, copy_type, pad; // copy_type 0: no copy
+    float decay;
+    int pad2;
+};
+struct wdg_adamw_batch {
+    std::vector<WdgAdamwChunk> chunks;
+    int bits = 32;
+    const WdgAdamwChunk* table = nullptr;         // device memory of the caller
+};
+
+// the step's numbers as the kernel takes them
+struct WdgAdamwHyper {
+    float b1, c1, b2, c2;                         // beta, 1 - beta
+    float eps, lr_wd, lr;
+    float lr_bc1, rbc2;                           // lr / (1 - beta1^t), 1 / sqrt(1 - beta2^t), when t is known on the host
+    double log_b1, log_b2;                        // ... otherwise they come from t in device memory
+    const long long* step_dev;
+    double grad_scale, max_norm;
+    const double* parts;                          // partial sums of g^2, or NULL: no clipping
+    int nparts;
+    float* norm;
+};
+
+// ---- four elements of a tensor, the missing ones of its last quad read as zero ----------------------------------------------------
+template <class T>
+__device__ __forceinline__ f32x4 wdg_aw_load(const T* p, int n) {
+    f32x4 r = {0.f, 0.f, 0.f, 0.f};
+    if (n >= 4) {
+        const WdgVec<T, 4> v = wdg_vec_load<T, 4>(p);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) r[j] = (float)v.e[j];
+    } else {
+#pragma unroll
+        for (int j = 0; j < 3; ++j)
+            if (j < n) r[j] = (float)p[j];
+    }
+    return r;
+}
+template <class T>
+__device__ __forceinline__ void wdg_aw_store(T* p, int n, const f32x4& r) {
+    if (n >= 4) {
+        WdgVec<T, 4> v;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v.e[j] = (T)r[j];
+        wdg_vec_store<T, 4>(p, v);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 3; ++j)
+            if (j < n) p[j] = (T)r[j];
+    }
+}
+
+// largest of 64 lanes' unsigned values, in every lane
+__device__ __forceinline__ unsigned wdg_wave_umax(unsigned v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v = max(v, (unsigned)__shfl_xor((int)v, o, 64));
+    return v;
+}
+// A block's scale from the largest bit pattern of its magnitudes (as integers: above infinity come the NaNs, which a float maximum would
+// drop).  inv = 1 / scale, 0 where the block holds zeros alone; a block that is not finite gets a NaN for its scale.
+__device__ __forceinline__ float wdg_aw_scale(unsigned bits, float& inv) {
+    if (bits >= 0x7f800000u) {
+        inv = 0.f;
+        return __builtin_nanf("");
+    }
+    if (bits < 0x00800000u) {                     // below 2^-126: its reciprocal would not be a number
+        inv = 0.f;
+        return 0.f;
+    }
+    const float s = __builtin_bit_cast(float, bits);
+    inv = 1.f / s;
+    return s;
+}
+
+// clipping: the gradients' factor grad_scale c, the same bits in every workgroup (all add the same numbers in the same order); false
+// where the norm is not finite.  All threads call it.
+__device__ __forceinline__ bool wdg_aw_clip(const WdgAdamwHyper& h, double* red, float& gs) {
+    gs = (float)h.grad_scale;
+    if (!h.parts) return true;
+    double s = 0.0;
+    for (int i = threadIdx.x; i < h.nparts; i += 256) s += h.parts[i];
+    s = wdg_wave_sum_d(s);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+    __syncthreads();
+    const double norm = h.grad_scale * sqrt((red[0] + red[1]) + (red[2] + red[3]));
+    if (h.norm && blockIdx.x == 0 && threadIdx.x == 0) h.norm[0] = (float)norm;
+    if (!(norm <= 1.7976931348623157e308)) return false;
+    gs = (float)(h.grad_scale * (h.max_norm / fmax(norm, h.max_norm)));
+    return true;
+}
+
+template <int BITS, class PT, class GT>
+__device__ __forceinline__ void wdg_aw_chunk(const WdgAdamwChunk& q, const WdgAdamwHyper& h, float gs, float lr_bc1, float rbc2) {
+    const float keep = 1.f - h.lr_wd * q.decay;
+    PT* p = static_cast<PT*>(q.p);
+    const GT* g = static_cast<const GT*>(q.g);
+    const int lane = threadIdx.x & 63;
+#pragma unroll 1
+    for (int i = 0; i < AW_CHUNK / 1024; ++i) {
+        const int e = (i * 256 + (int)threadIdx.x) * 4;
+        if (i * 1024 + ((int)threadIdx.x & ~63) * 4 >= q.n) break;        // (the wave's whole block lies behind the tensor)
+        const int n = q.n - e;                                           // elements from here on; may be negative for the last lanes
+        f32x4 w = wdg_aw_load(p + e, n);
+        const f32x4 gr = wdg_aw_load(g + e, n);
+        f32x4 m, v;
+        if constexpr (BITS == 32) {
+            m = wdg_aw_load(static_cast<const float*>(q.m) + e, n);
+            v = wdg_aw_load(static_cast<const float*>(q.v) + e, n);
+        } else {
+            const unsigned cm = static_cast<const unsigned*>(q.m)[e >> 2], cv = static_cast<const unsigned*>(q.v)[e >> 2];
+            const float sm = q.ms[e / AW_BLOCK] * (1.f / (127.f * 127.f)), sv = q.vs[e / AW_BLOCK];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float a = (float)(signed char)(cm >> (8 * j)), b = (float)((cv >> (8 * j)) & 255u) * (1.f / 255.f);
+                m[j] = a * fabsf(a) * sm;
+                v[j] = (b * b) * (b * b) * sv;
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float gj = gr[j] * gs;
+            m[j] = h.b1 * m[j] + h.c1 * gj;
+            v[j] = h.b2 * v[j] + h.c2 * (gj * gj);
+            w[j] = w[j] * keep - lr_bc1 * (m[j] / (sqrtf(v[j]) * rbc2 + h.eps));
+        }
+        wdg_aw_store(p + e, n, w);
+        if (q.copy_type == WDG_BF16) wdg_aw_store(static_cast<__bf16*>(q.copy) + e, n, w);
+        else if (q.copy_type == WDG_F16) wdg_aw_store(static_cast<_Float16*>(q.copy) + e, n, w);
+        if constexpr (BITS == 32) {
+            wdg_aw_store(static_cast<float*>(q.m) + e, n, m);
+            wdg_aw_store(static_cast<float*>(q.v) + e, n, v);
+        } else {
+            unsigned tm = 0, tv = 0;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float a = m[j], b = v[j];           // (a bit cast of a vector's element would take element 0)
+                tm = max(tm, j < n ? __builtin_bit_cast(unsigned, a) & 0x7fffffffu : 0u);
+                tv = max(tv, j < n ? __builtin_bit_cast(unsigned, b) & 0x7fffffffu : 0u);
+            }
+            float im, iv;
+            const float sm = wdg_aw_scale(wdg_wave_umax(tm), im), sv = wdg_aw_scale(wdg_wave_umax(tv), iv);
+            unsigned cm = 0, cv = 0;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (j >= n) continue;
+                // both companding roots on the hardware square root (one unit in the last place of a value that is rounded to 1 / 127
+                // or 1 / 255): only a value that close to the border between two codes can take the other one
+                const float a = rintf(127.f * __builtin_amdgcn_sqrtf(fabsf(m[j]) * im));
+                float b = rintf(255.f * __builtin_amdgcn_sqrtf(__builtin_amdgcn_sqrtf(v[j] * iv)));
+                b = v[j] * iv > 0.f ? fmaxf(b, 1.f) : 0.f;
+                const int ai = im > 0.f ? (int)(m[j] < 0.f ? -a : a) : 0, bi = iv > 0.f ? (int)b : 0;
+                cm |= ((unsigned)ai & 255u) << (8 * j);
+                cv |= ((unsigned)bi & 255u) << (8 * j);
+            }
+            static_cast<unsigned*>(q.m)[e >> 2] = cm;
+            static_cast<unsigned*>(q.v)[e >> 2] = cv;
+            if (lane == 0) {
+                q.ms[e / AW_BLOCK] = sm;
+                q.vs[e / AW_BLOCK] = sv;
+            }
+        }
+    }
+}
+
+template <int BITS, class PT>
+__device__ __forceinline__ void wdg_aw_by_grad(const WdgAdamwChunk& q, const WdgAdamwHyper& h, float gs, float lr_bc1, float rbc2) {
+    if (q.g_type == WDG_F32) wdg_aw_chunk<BITS, PT, float>(q, h, gs, lr_bc1, rbc2);
+    else if (q.g_type == WDG_BF16) wdg_aw_chunk<BITS, PT, __bf16>(q, h, gs, lr_bc1, rbc2);
+    else wdg_aw_chunk<BITS, PT, _Float16>(q, h, gs, lr_bc1, rbc2);
+}
+
+template <int BITS>
+__global__ void __launch_bounds__(256) wdg_adamw_kernel(const WdgAdamwChunk* __restrict__ table, const WdgAdamwHyper h) {
+    __shared__ double red[4];
+    const WdgAdamwChunk q = table[blockIdx.x];
+    float gs, lr_bc1 = h.lr_bc1, rbc2 = h.rbc2;
+    if (h.step_dev) {
+        // 1 - beta^t = -expm1(t log beta): the difference keeps its digits when beta^t is close to 1
+        const double t = (double)*h.step_dev;
+        lr_bc1 = h.lr / -expm1f((float)(t * h.log_b1));
+        rbc2 = 1.f / sqrtf(-expm1f((float)(t * h.log_b2)));
+    }
+    if (!wdg_aw_clip(h, red, gs)) return;
+    if (q.p_type == WDG_F32) wdg_aw_by_grad<BITS, float>(q, h, gs, lr_bc1, rbc2);
+    else if (q.p_type == WDG_BF16) wdg_aw_by_grad<BITS, __bf16>(q, h, gs, lr_bc1, rbc2);
+    else wdg_aw_by_grad<BITS, _Float16>(q, h, gs, lr_bc1, rbc2);
+}
+
+// ---- sum of g^2 over all chunks: AW_PARTS workgroups, each every AW_PARTS-th chunk; fp64, since a square leaves fp32's range where the
+// gradient itself does not -----------------------------------------------------------------------------------------------------------
+template <class GT>
+__device__ __forceinline__ double wdg_aw_sumsq(const GT* g, int n) {
+    double s = 0.0;
+    for (int e = (int)threadIdx.x * 4; e < n; e += 1024) {
+        const f32x4 v = wdg_aw_load(g + e, n - e);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s += (double)v[j] * (double)v[j];
+    }
+    return s;
+}
+__global__ void __launch_bounds__(256) wdg_adamw_sumsq_kernel(const WdgAdamwChunk* __restrict__ table, int chunks, double* parts) {
+    __shared__ double red[4];
+    double s = 0.0;
+    for (int c = blockIdx.x; c < chunks; c += gridDim.x) {
+        const WdgAdamwChunk q = table[c];
+        if (q.g_type == WDG_F32) s += wdg_aw_sumsq(static_cast<const float*>(q.g), q.n);
+        else if (q.g_type == WDG_BF16) s += wdg_aw_sumsq(static_cast<const __bf16*>(q.g), q.n);
+        else s += wdg_aw_sumsq(static_cast<const _Float16*>(q.g), q.n);
+    }
+    s = wdg_wave_sum_d(s);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) parts[blockIdx.x] = (red[0] + red[1]) + (red[2] + red[3]);
+}
+__global__ void __launch_bounds__(256) wdg_adamw_norm_kernel(const double* __restrict__ parts, int nparts, double scale, float* norm) {
+    __shared__ double red[4];
+    double s = 0.0;
+    for (int i = threadIdx.x; i < nparts; i += 256) s += parts[i];
+    s = wdg_wave_sum_d(s);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) norm[0] = (float)(scale * sqrt((red[0] + red[1]) + (red[2] + red[3])));
+}
+
+// ---- the values behind 8-bit states: four codes per thread, blockIdx.y 0 the first moment, 1 the second ----------------------------
+template <class T>
+__global__ void __launch_bounds__(256) wdg_adamw_moments_kernel(const unsigned* m, const float* ms, const unsigned* v, const float* vs, T* mo,
+                                                                T* vo, long long quads) {
+    const bool second = blockIdx.y == 1;
+    T* out = second ? vo : mo;
+    if (!out) return;
+    const unsigned* codes = second ? v : m;
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < quads; i += (long long)gridDim.x * 256) {
+        const unsigned c = codes[i];
+        const float s = (second ? vs : ms)[i / (AW_BLOCK / 4)];
+        f32x4 r;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float a = (float)(signed char)(c >> (8 * j)), b = (float)((c >> (8 * j)) & 255u) * (1.f / 255.f);
+            r[j] = second ? (b * b) * (b * b) * s : a * fabsf(a) * (s * (1.f / (127.f * 127.f)));
+        }
+        wdg_aw_store(out + 4 * i, 4, r);
+    }
+}
+
+// ---- host side ---------------------------------------------------------------------------------------------------------------------
+static int aw_bytes(int type) { return type == WDG_F32 ? 4 : 2; }
+static bool aw_aligned(const void* p, int a) { return ((uintptr_t)p & (uintptr_t)(a - 1)) == 0; }
+
+// NULL, or what is wrong with tensor t
+static const char* aw_check(const wdg_adamw_tensor& t, int bits) {
+    if (t.n < 0) return "negative size";
+    if (t.p_type < WDG_F32 || t.p_type > WDG_F16 || t.g_type < WDG_F32 || t.g_type > WDG_F16) return "unknown type";
+    if (t.copy && t.copy_type != WDG_BF16 && t.copy_type != WDG_F16) return "the copy is bf16 or fp16";
+    if (!(t.decay >= 0.f) || t.decay > 3.4e38f) return "decay factor";
+    if (t.n == 0) return nullptr;
+    if (!t.p || !t.g || !t.m || !t.v || (bits == 8 && (!t.m_scale || !t.v_scale))) return "null pointer";
+    if (!aw_aligned(t.p, aw_bytes(t.p_type)) || !aw_aligned(t.g, aw_bytes(t.g_type)) || !aw_aligned(t.copy, 2) || !aw_aligned(t.m, 4) ||
+        !aw_aligned(t.v, 4) || !aw_aligned(t.m_scale, 4) || !aw_aligned(t.v_scale, 4))
+        return "not aligned to its element";
+    return nullptr;
+}
+
+struct AwRange {
+    uintptr_t begin, end;
+    bool written;
+};
+
+static int aw_create(wdg_adamw_batch** out, const wdg_adamw_tensor* tensors, int n, int bits) {
+    std::vector<AwRange> ranges;
+    int64_t chunks = 0;
+    for (int i = 0; i < n; ++i) {
+        const wdg_adamw_tensor& t = tensors[i];
+        if (const char* why = aw_check(t, bits)) {
+            wdg_set_error("wdg_adamw_create: tensor %d: %s", i, why);
+            return WDG_ERR_ARG;
+        }
+        if (t.n == 0) continue;
+        const int64_t blocks = (t.n + AW_BLOCK - 1) / AW_BLOCK;
+        auto add = [&](const void* p, int64_t bytes, bool written) {
+            if (p) ranges.push_back({(uintptr_t)p, (uintptr_t)p + (uintptr_t)bytes, written});
+        };
+        add(t.p, t.n * aw_bytes(t.p_type), true);
+        add(t.g, t.n * aw_bytes(t.g_type), false);
+        add(t.copy, t.n * 2, true);
+        add(t.m, bits == 8 ? blocks * AW_BLOCK : t.n * 4, true);
+        add(t.v, bits == 8 ? blocks * AW_BLOCK : t.n * 4, true);
+        if (bits == 8) {
+            add(t.m_scale, blocks * 4, true);
+            add(t.v_scale, blocks * 4, true);
+        }
+        chunks += (t.n + AW_CHUNK - 1) / AW_CHUNK;
+    }
+    if (chunks > 0x7fffffff) {
+        wdg_set_error("wdg_adamw_create: more than 2^31 chunks of %d elements", AW_CHUNK);
+        return WDG_ERR_ARG;
+    }
+    // in address order, a range may only begin where every written one before it — and, if it is written itself, every one — has ended
+    std::sort(ranges.begin(), ranges.end(), [](const AwRange& a, const AwRange& b) { return a.begin < b.begin; });
+    uintptr_t end_written = 0, end_any = 0;
+    for (const AwRange& r : ranges) {
+        if (r.begin < (r.written ? end_any : end_written)) {
+            wdg_set_error("wdg_adamw_create: tensors overlap (the same one twice, a gradient over a weight or a state of two tensors)");
+            return WDG_ERR_ARG;
+        }
+        end_any = std::max(end_any, r.end);
+        if (r.written) end_written = std::max(end_written, r.end);
+    }
+    wdg_adamw_batch* b = new wdg_adamw_batch();
+    b->bits = bits;
+    try {
+        b->chunks.reserve((size_t)chunks);
+    } catch (...) {
+        delete b;
+        throw;
+    }
+    for (int i = 0; i < n; ++i) {
+        const wdg_adamw_tensor& t = tensors[i];
+        for (int64_t e = 0; e < t.n; e += AW_CHUNK) {
+            WdgAdamwChunk q;
+            memset(&q, 0, sizeof(q));
+            q.p = (char*)t.p + e * aw_bytes(t.p_type);
+            q.g = (const char*)t.g + e * aw_bytes(t.g_type);
+            q.m = (char*)t.m + e * (bits == 8 ? 1 : 4);
+            q.v = (char*)t.v + e * (bits == 8 ? 1 : 4);
+            q.ms = bits == 8 ? t.m_scale + e / AW_BLOCK : nullptr;
+            q.vs = bits == 8 ? t.v_scale + e / AW_BLOCK : nullptr;
+            q.copy = t.copy ? (char*)t.copy + e * 2 : nullptr;
+            q.n = (int)std::min<int64_t>(AW_CHUNK, t.n - e);
+            q.p_type = (unsigned char)t.p_type;
+            q.g_type = (unsigned char)t.g_type;
+            q.copy_type = t.copy ? (unsigned char)t.copy_type : 0;
+            q.decay = t.decay;
+            b->chunks.push_back(q);
+        }
+    }
+    *out = b;
+    return WDG_OK;
+}
+
+extern "C" int wdg_adamw_create(wdg_adamw_batch** out, const wdg_adamw_tensor* tensors, int n, int state_bits) {
+    WDG_CHECK_ARG(out && n >= 0 && (tensors || n == 0), "bad argument");
+    WDG_CHECK_ARG(state_bits == 32 || state_bits == 8, "states are held in 32 or 8 bits");
+    try {
+        return aw_create(out, tensors, n, state_bits);
+    } catch (const std::exception& e) {
+        wdg_set_error("wdg_adamw_create: %s", e.what());
+        return WDG_ERR_ARG;
+    }
+}
+
+extern "C" size_t wdg_adamw_table_bytes(const wdg_adamw_batch* b) { return b ? b->chunks.size() * sizeof(WdgAdamwChunk) : 0; }
+
+extern "C" int wdg_adamw_bind(wdg_adamw_batch* b, void* table, size_t table_bytes, wdg_stream stream) {
+    WDG_CHECK_ARG(b, "null batch");
+    if (b->chunks.empty()) return WDG_OK;
+    WDG_CHECK_ARG(table && aw_aligned(table, 16) && table_bytes >= wdg_adamw_table_bytes(b), "table: wdg_adamw_table_bytes() of device memory, 16-byte aligned");
+    WDG_HIP(hipMemcpyAsync(table, b->chunks.data(), wdg_adamw_table_bytes(b), hipMemcpyHostToDevice, (hipStream_t)stream));
+    WDG_HIP(hipStreamSynchronize((hipStream_t)stream));
+    b->table = (const WdgAdamwChunk*)table;
+    return WDG_OK;
+}
+
+extern "C" int wdg_adamw_destroy(wdg_adamw_batch* b) {
+    delete b;
+    return WDG_OK;
+}
+
+extern "C" size_t wdg_adamw_scratch_bytes(void) { return AW_PARTS * sizeof(double); }
+
+static int aw_parts(const wdg_adamw_batch* b) { return (int)std::min<size_t>(AW_PARTS, b->chunks.size()); }
+
+static int aw_sumsq(const wdg_adamw_batch* b, double* parts, hipStream_t st) {
+    if (aw_parts(b) == 0) return WDG_OK;
+    hipLaunchKernelGGL(wdg_adamw_sumsq_kernel, dim3(aw_parts(b)), dim3(256), 0, st, b->table, (int)b->chunks.size(), parts);
+    WDG_LAUNCH_CHECK();
+    return WDG_OK;
+}
+
+static int aw_norm(const wdg_adamw_batch* b, double scale, float* norm, const double* parts, hipStream_t st) {
+    hipLaunchKernelGGL(wdg_adamw_norm_kernel, dim3(1), dim3(256), 0, st, parts, aw_parts(b), scale, norm);
+    WDG_LAUNCH_CHECK();
+    return WDG_OK;
+}
+
+extern "C" int wdg_adamw_grad_norm(const wdg_adamw_batch* b, double grad_scale, float* norm, void* scratch, size_t scratch_bytes,
+                                   wdg_stream stream) {
+    WDG_CHECK_ARG(b && norm, "null argument");
+    WDG_CHECK_ARG(b->chunks.empty() || b->table, "wdg_adamw_bind has not been called");
+    WDG_CHECK_ARG(grad_scale >= 0.0 && grad_scale < INFINITY, "gradient scale");
+    if (!scratch || !aw_aligned(scratch, 8) || scratch_bytes < wdg_adamw_scratch_bytes()) {
+        wdg_set_error("wdg_adamw_grad_norm: scratch too small or not aligned");
+        return WDG_ERR_WORKSPACE;
+    }
+    const int rc = aw_sumsq(b, (double*)scratch, (hipStream_t)stream);
+    return rc != WDG_OK ? rc : aw_norm(b, grad_scale, norm, (const double*)scratch, (hipStream_t)stream);
+}
+
+extern "C" int wdg_adamw_step(const wdg_adamw_batch* b, const wdg_adamw_args* a, void* scratch, size_t scratch_bytes, wdg_stream stream) {
+    WDG_CHECK_ARG(b && a, "null argument");
+    WDG_CHECK_ARG(b->chunks.empty() || b->table, "wdg_adamw_bind has not been called");
+    WDG_CHECK_ARG(a->beta1 >= 0.0 && a->beta1 < 1.0 && a->beta2 >= 0.0 && a->beta2 < 1.0, "beta1 and beta2 have to be in [0, 1)");
+    WDG_CHECK_ARG(a->eps >= 0.0 && a->lr >= 0.0 && a->weight_decay >= 0.0 && a->grad_scale >= 0.0 && a->eps < INFINITY && a->lr < INFINITY &&
+                      a->weight_decay < INFINITY && a->grad_scale < INFINITY && a->max_norm < INFINITY, "lr, eps, weight decay and gradient scale: finite, not negative");
+    WDG_CHECK_ARG(a->step_dev || a->step >= 1, "steps count from 1");
+    const bool clip = a->max_norm > 0.0;
+    hipStream_t st = (hipStream_t)stream;
+    if (clip && (!scratch || !aw_aligned(scratch, 8) || scratch_bytes < wdg_adamw_scratch_bytes())) {
+        wdg_set_error("wdg_adamw_step: scratch too small or not aligned");
+        return WDG_ERR_WORKSPACE;
+    }
+    if (b->chunks.empty()) return clip && a->norm ? aw_norm(b, 0.0, a->norm, (const double*)scratch, st) : WDG_OK;
+    if (clip) {
+        const int rc = aw_sumsq(b, (double*)scratch, st);
+        if (rc != WDG_OK) return rc;
+    }
+    WdgAdamwHyper h;
+    memset(&h, 0, sizeof(h));
+    h.b1 = (float)a->beta1;
+    h.c1 = (float)(1.0 - a->beta1);
+    h.b2 = (float)a->beta2;
+    h.c2 = (float)(1.0 - a->beta2);
+    h.eps = (float)a->eps;
+    h.lr = (float)a->lr;
+    h.lr_wd = (float)(a->lr * a->weight_decay);
+    h.step_dev = (const long long*)a->step_dev;
+    if (a->step_dev) {
+        h.log_b1 = log(a->beta1);                  // (beta = 0: -inf, and 1 - beta^t = 1)
+        h.log_b2 = log(a->beta2);
+    } else {
+        h.lr_bc1 = (float)(a->lr / (1.0 - pow(a->beta1, (double)a->step)));
+        h.rbc2 = (float)(1.0 / sqrt(1.0 - pow(a->beta2, (double)a->step)));
+    }
+    h.grad_scale = a->grad_scale;
+    if (clip) {
+        h.max_norm = a->max_norm;
+        h.parts = (const double*)scratch;
+        h.nparts = aw_parts(b);
+        h.norm = a->norm;
+    }
+    const dim3 grid((unsigned)b->chunks.size());
+    if (b->bits == 32) hipLaunchKernelGGL(wdg_adamw_kernel<32>, grid, dim3(256), 0, st, b->table, h);
+    else hipLaunchKernelGGL(wdg_adamw_kernel<8>, grid, dim3(256), 0, st, b->table, h);
+    WDG_LAUNCH_CHECK();
+    return WDG_OK;
+}
+
+extern "C" int wdg_adamw_moments(const void* m, const float* m_scale, const void* v, const float* v_scale, int64_t blocks, void* m_out,
+                                 void* v_out, int out_type, wdg_stream stream) {
+    WDG_CHECK_ARG(blocks >= 0 && out_type >= WDG_F32 && out_type <= WDG_F16, "bad argument");
+    if (blocks == 0 || (!m_out && !v_out)) return WDG_OK;
+    WDG_CHECK_ARG((!m_out || (m && m_scale)) && (!v_out || (v && v_scale)), "null argument");
+    WDG_CHECK_ARG(aw_aligned(m, 4) && aw_aligned(v, 4) && aw_aligned(m_out, aw_bytes(out_type)) && aw_aligned(v_out, aw_bytes(out_type)), "alignment");
+    const long long quads = blocks * (AW_BLOCK / 4);
+    const dim3 grid((unsigned)std::min<long long>((quads + 255) / 256, 8192), 2);
+    hipStream_t st = (hipStream_t)stream;
+    const unsigned *mc = (const unsigned*)m, *vc = (const unsigned*)v;
+    if (out_type == WDG_F32) hipLaunchKernelGGL(wdg_adamw_moments_kernel<float>, grid, dim3(256), 0, st, mc, m_scale, vc, v_scale, (float*)m_out, (float*)v_out, quads);
+    else if (out_type == WDG_BF16) hipLaunchKernelGGL(wdg_adamw_moments_kernel<__bf16>, grid, dim3(256), 0, st, mc, m_scale, vc, v_scale, (__bf16*)m_out, (__bf16*)v_out, quads);
+    else hipLaunchKernelGGL(wdg_adamw_moments_kernel<_Float16>, grid, dim3(256), 0, st, mc, m_scale, vc, v_scale, (_Float16*)m_out, (_Float16*)v_out, quads);
+    WDG_LAUNCH_CHECK();
+    return WDG_OK;
+}

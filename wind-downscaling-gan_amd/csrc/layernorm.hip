@@ -12,26 +12,9 @@
 // Numerics: statistics, sums and the normalised value are fp32 whatever the tensors' type; z and dx are rounded once, on store.  The
 // mean is corrected by the mean of (x - mean), which is what fp32 left out of it, so a row with an offset of many standard deviations
 // keeps its digits; the variance is the sum of squares about the corrected mean.
-#include "common.h"
+#include "vec.h"
 #include <algorithm>
 
-// ---- element and vector access ------------------------------------------------------------------------------------------------
-// V elements in one request.  Rows may start at any element (odd widths, views into wider buffers), so no alignment beyond the
-// element's own is promised; the global memory path of this target takes such requests whole.
-template <class T, int V>
-struct WdgVec {
-    T e[V];
-};
-template <class T, int V>
-__device__ __forceinline__ WdgVec<T, V> wdg_vec_load(const T* p) {
-    WdgVec<T, V> v;
-    __builtin_memcpy(&v, p, sizeof(v));
-    return v;
-}
-template <class T, int V>
-__device__ __forceinline__ void wdg_vec_store(T* p, const WdgVec<T, V>& v) {
-    __builtin_memcpy(p, &v, sizeof(v));
-}
 // parameter c of gamma / beta: fp32 (ptype 0) or the 16-bit type of the activations; a missing vector reads as `none`
 template <class T>
 __device__ __forceinline__ float wdg_ln_param(const void* p, int ptype, int64_t c, float none) {

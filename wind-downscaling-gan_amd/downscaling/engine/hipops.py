@@ -186,6 +186,130 @@ class _PrepBatch:
             pass
 
 
+class _AdamWBatch:
+    """AdamW over a list of tensors (HipOps.make_adamw): one launch per step, two with clipping.  The tensors' addresses are fixed:
+    gradients are written in place between steps, and the batch has to outlive every graph that captured one of its calls.
+
+    State layout: tensor i's states start at `offsets[i]`, a multiple of 256, of flat buffers of `total` elements (a multiple of 256):
+    `m`, `v` in fp32, or as int8 / uint8 codes with `m_scale`, `v_scale` [total / 256] (wdg_adamw_step in include/wdgan.h)."""
+    BLOCK = 256
+
+    def __init__(self, ops, entries, state_bits=32, state=None):
+        if state_bits not in (32, 8):
+            raise ValueError(f"states are held in 32 or 8 bits, not {state_bits}")
+        if ops.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("make_adamw lays out and copies a table: not while a graph is captured")
+        self.ops, self.state_bits = ops, state_bits
+        self.entries = [tuple(e) + (None,) * (4 - len(e)) for e in entries]
+        self.offsets, off = [], 0
+        for p, g, decay, copy in self.entries:
+            ops._on_device(p, g, copy)
+            for name, t, dtypes in (("weights", p, ops.TYPES), ("gradient", g, ops.TYPES), ("copy", copy, (torch.bfloat16, torch.float16))):
+                if t is None and name == "copy":
+                    continue
+                if t.dtype not in dtypes or t.shape != p.shape or not t.is_contiguous():
+                    raise ValueError(f"{name}: a contiguous {tuple(p.shape)} tensor of {' or '.join(str(d) for d in dtypes)} is wanted, got {t.dtype} {tuple(t.shape)}")
+            self.offsets.append(off)
+            off += -(-p.numel() // self.BLOCK) * self.BLOCK
+        self.total = off
+        kinds = [(torch.float32, off)] * 2 if state_bits == 32 else [(torch.int8, off), (torch.uint8, off)] + [(torch.float32, off // self.BLOCK)] * 2
+        if state is None:
+            state = [torch.zeros(n, dtype=d, device=ops.device) for d, n in kinds]
+        state = list(state)
+        ops._on_device(*state)
+        if len(state) != len(kinds) or any(t.dtype != d or tuple(t.shape) != (n,) or not t.is_contiguous() for t, (d, n) in zip(state, kinds)):
+            raise ValueError("state: flat contiguous tensors " + ", ".join(f"{d} [{n}]" for d, n in kinds) + " are wanted")
+        self.state = state
+        self.m, self.v = state[:2]
+        self.m_scale, self.v_scale = state[2:] if state_bits == 8 else (None, None)
+        self.handle = None
+        arr = (native.AdamWTensor * max(len(self.entries), 1))()
+        for i, ((p, g, decay, copy), o) in enumerate(zip(self.entries, self.offsets)):
+            at = lambda t, k: 0 if t is None else t.data_ptr() + k * t.element_size()      # noqa: E731
+            arr[i] = native.AdamWTensor(p.data_ptr(), g.data_ptr(), at(self.m, o), at(self.v, o), at(self.m_scale, o // self.BLOCK),
+                                        at(self.v_scale, o // self.BLOCK), _ptr(copy), p.numel(), ops.TYPES[p.dtype], ops.TYPES[g.dtype],
+                                        0 if copy is None else ops.TYPES[copy.dtype], float(decay))
+        handle = C.c_void_p()
+        native.check(ops.lib.wdg_adamw_create(C.byref(handle), arr, len(self.entries), state_bits), "adamw_create")
+        self.handle = handle
+        self.scratch_bytes = int(ops.lib.wdg_adamw_scratch_bytes())
+        need = int(ops.lib.wdg_adamw_table_bytes(handle))
+        self.table = torch.empty(max(need, 16), dtype=torch.uint8, device=ops.device)
+        self.home = ops.stream
+        with torch.cuda.device(ops.device):
+            native.check(ops.lib.wdg_adamw_bind(handle, self.table.data_ptr(), need, self.home), "adamw_bind")
+
+    def _launch(self):
+        """(scratch, stream) of one call: the scratch is the call's own (the allocator orders its reuse on this stream, and inside a
+        graph capture it belongs to the graph); what the batch owns is kept from reuse while another stream than its own works on it."""
+        stream = self.ops.stream
+        if stream != self.home and not torch.cuda.is_current_stream_capturing():
+            for t in (self.table, *self.state):
+                t.record_stream(torch.cuda.current_stream(self.ops.device))
+        return torch.empty(self.scratch_bytes // 8, dtype=torch.float64, device=self.ops.device), stream
+
+    def _norm_ptr(self, norm):
+        if norm is not None:
+            self.ops._on_device(norm)
+            if norm.dtype != torch.float32 or norm.numel() != 1:
+                raise ValueError(f"norm: one fp32 value is wanted, got {norm.dtype} {tuple(norm.shape)}")
+        return _ptr(norm)
+
+    def step(self, t, lr, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=0.0, grad_scale=1.0, max_norm=None, norm=None):
+        """One AdamW step, the t-th (t = 1, 2, ...; an int, or an int64 device tensor of one element that a captured step reads when it is
+        replayed).  grad_scale multiplies every gradient; max_norm clips their global norm, which goes to `norm` (one fp32 value on the
+        device) — a norm that is not finite leaves everything as it was."""
+        args = native.AdamWArgs(lr, beta1, beta2, eps, weight_decay, grad_scale, 0.0 if max_norm is None else max_norm, 0, 0, self._norm_ptr(norm))
+        if max_norm is None and norm is not None:
+            raise ValueError("norm is formed with max_norm only (grad_norm forms it alone)")
+        if max_norm is not None and not max_norm > 0:
+            raise ValueError("max_norm has to be above zero")
+        if torch.is_tensor(t):
+            self.ops._on_device(t)
+            if t.dtype != torch.int64 or t.numel() != 1:
+                raise ValueError(f"t: an int or one int64 value on the device is wanted, got {t.dtype} {tuple(t.shape)}")
+            args.step_dev = t.data_ptr()
+        else:
+            args.step = t
+        with torch.cuda.device(self.ops.device):
+            scratch, stream = self._launch()
+            native.check(self.ops.lib.wdg_adamw_step(self.handle, C.byref(args), scratch.data_ptr(), self.scratch_bytes, stream), "adamw_step")
+
+    def grad_norm(self, norm, grad_scale=1.0):
+        """norm[0] = grad_scale * sqrt(sum of all gradients' squares), on the device."""
+        if norm is None:
+            raise ValueError("norm: one fp32 value is wanted")
+        p = self._norm_ptr(norm)
+        with torch.cuda.device(self.ops.device):
+            scratch, stream = self._launch()
+            native.check(self.ops.lib.wdg_adamw_grad_norm(self.handle, grad_scale, p, scratch.data_ptr(), self.scratch_bytes, stream), "adamw_grad_norm")
+
+    def moments(self, m_out=None, v_out=None):
+        """The moments as numbers, in the state's flat layout: into m_out / v_out ([total], one type of fp32, bf16, fp16)."""
+        outs = [t for t in (m_out, v_out) if t is not None]
+        self.ops._on_device(*outs)
+        if any(t.dtype not in self.ops.TYPES or t.dtype != outs[0].dtype or tuple(t.shape) != (self.total,) or not t.is_contiguous() for t in outs):
+            raise ValueError(f"contiguous [{self.total}] tensors of one type of {', '.join(str(d) for d in self.ops.TYPES)} are wanted")
+        if self.state_bits == 32:
+            for t, s in ((m_out, self.m), (v_out, self.v)):
+                if t is not None:
+                    t.copy_(s)
+            return
+        if not outs:
+            return
+        with torch.cuda.device(self.ops.device):
+            native.check(self.ops.lib.wdg_adamw_moments(self.m.data_ptr(), self.m_scale.data_ptr(), self.v.data_ptr(), self.v_scale.data_ptr(),
+                                                        self.total // self.BLOCK, _ptr(m_out), _ptr(v_out), self.ops.TYPES[outs[0].dtype],
+                                                        self.ops.stream), "adamw_moments")
+
+    def __del__(self):
+        try:
+            if self.handle is not None:
+                self.ops.lib.wdg_adamw_destroy(self.handle)
+        except Exception:
+            pass
+
+
 class _Fork:
     def __init__(self, ops, name="side", stream=None):
         self.ops = ops
@@ -1421,3 +1545,10 @@ class HipOps:
     def adam_tf(self, p, g, m, v, lr_t, beta1, beta2, eps, grad_scale=1.0):
         native.check(self.lib.wdg_adam_tf(p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), p.numel(), lr_t,
                                           beta1, beta2, eps, grad_scale, self.stream), "adam_tf")
+
+    def make_adamw(self, entries, state_bits=32, state=None):
+        """AdamW over many tensors: entries = [(weights, gradient, decay factor[, 16-bit copy of the weights])], contiguous tensors of one
+        shape each, weights and gradients fp32, bf16 or fp16; states of 32 or 8 bits per moment and element, zero or adopted (`state`:
+        (m, v) or (m, v, m_scale, v_scale) in the layout of _AdamWBatch, for instance another batch's).  Returns an object with step(),
+        grad_norm() and moments()."""
+        return _AdamWBatch(self, entries, state_bits, state)

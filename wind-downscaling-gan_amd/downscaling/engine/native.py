@@ -30,6 +30,21 @@ class PrepLayer(C.Structure):
 
 PREP_SN, PREP_PACK_ALL = 1, 2
 
+
+class AdamWTensor(C.Structure):
+    _fields_ = [
+        ("p", c_fp), ("g", c_fp), ("m", c_fp), ("v", c_fp), ("m_scale", c_fp), ("v_scale", c_fp), ("copy", c_fp),
+        ("n", i64), ("p_type", i32), ("g_type", i32), ("copy_type", i32), ("decay", f32),
+    ]
+
+
+class AdamWArgs(C.Structure):
+    _fields_ = [
+        ("lr", f64), ("beta1", f64), ("beta2", f64), ("eps", f64), ("weight_decay", f64), ("grad_scale", f64), ("max_norm", f64),
+        ("step", i64), ("step_dev", c_fp), ("norm", c_fp),
+    ]
+
+
 # name -> (restype, argtypes); every symbol of include/wdgan.h
 SIGNATURES = {
     "wdg_last_error": (C.c_char_p, []),
@@ -176,6 +191,14 @@ SIGNATURES = {
     "wdg_input_assemble_slots": (i32, [c_fp, i64, i64, i32, c_fp, i32, i64, i32, i32, i32, u64, u64, f32, i32, i32, c_fp]),
     "wdg_philox_uniform": (i32, [c_fp, i64, u64, u64, c_fp]),
     "wdg_adam_tf": (i32, [c_fp, c_fp, c_fp, c_fp, i64, f32, f32, f32, f32, f32, c_fp]),
+    "wdg_adamw_create": (i32, [C.POINTER(C.c_void_p), C.POINTER(AdamWTensor), i32, i32]),
+    "wdg_adamw_table_bytes": (szt, [C.c_void_p]),
+    "wdg_adamw_bind": (i32, [C.c_void_p, c_fp, szt, c_fp]),
+    "wdg_adamw_destroy": (i32, [C.c_void_p]),
+    "wdg_adamw_scratch_bytes": (szt, []),
+    "wdg_adamw_step": (i32, [C.c_void_p, C.POINTER(AdamWArgs), c_fp, szt, c_fp]),
+    "wdg_adamw_grad_norm": (i32, [C.c_void_p, f64, c_fp, c_fp, szt, c_fp]),
+    "wdg_adamw_moments": (i32, [c_fp, c_fp, c_fp, c_fp, i64, c_fp, c_fp, i32, c_fp]),
     "wdg_zero_ranges": (i32, [c_fp, C.POINTER(i64), i32, c_fp]),
 }
 

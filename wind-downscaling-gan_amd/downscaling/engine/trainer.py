@@ -32,6 +32,47 @@ class AdamTF:
         store.version += 1
 
 
+class AdamW:
+    """Adam with decoupled weight decay over the variables of one network (ops.make_adamw), an optimizer beside AdamTF:
+    p = p (1 - lr weight_decay d) - lr m_hat / (sqrt(v_hat) + epsilon), m_hat and v_hat corrected for their zero start (epsilon stands
+    inside that correction here, outside of it in AdamTF).
+
+    weight_decay applies to the variables that `decays(name)` accepts — by default kernels, not biases, gamma, beta.
+    global_clipnorm: the gradients of the whole network (after the data-parallel mean) are scaled so that their norm stays below it; a
+    step whose norm is not finite changes nothing but the step count.  state_bits = 8 holds both moments in a byte per element.
+    grad_norm: the last step's norm before clipping, on the device (None without global_clipnorm)."""
+
+    def __init__(self, lr=1e-3, beta_1=0.9, beta_2=0.999, epsilon=1e-8, weight_decay=0.01, global_clipnorm=None, state_bits=32, decays=None,
+                 learning_rate=None):
+        self.lr = float(learning_rate if learning_rate is not None else lr)
+        self.beta_1, self.beta_2, self.epsilon = float(beta_1), float(beta_2), float(epsilon)
+        self.weight_decay, self.state_bits = float(weight_decay), int(state_bits)
+        self.global_clipnorm = None if global_clipnorm is None else float(global_clipnorm)
+        if not (0 <= self.beta_1 < 1 and 0 <= self.beta_2 < 1 and self.epsilon >= 0 and self.weight_decay >= 0 and self.state_bits in (32, 8)
+                and (self.global_clipnorm is None or self.global_clipnorm > 0)):
+            raise ValueError("AdamW: betas in [0, 1), epsilon and weight_decay not negative, state_bits 32 or 8, global_clipnorm above zero")
+        self.decays = decays if decays is not None else (lambda name: name.rsplit("/", 1)[-1] in ("kernel", "recurrent_kernel", "w"))
+        self.iterations = 0
+        self.batch = self.grad_norm = self._store = None
+
+    def apply_gradients(self, store, grad_scale=1.0):
+        if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("AdamW.apply_gradients counts its steps on the host: a captured step would repeat one of them "
+                               "(ops.make_adamw(...).step takes a step count in device memory)")
+        if self.batch is None:
+            self._store = store
+            self.batch = store.ops.make_adamw([(v.value, v.grad, 1.0 if self.decays(v.name) else 0.0) for v in store.trainable], state_bits=self.state_bits)
+            if self.global_clipnorm is not None:
+                self.grad_norm = store.ops.zeros(1)
+        if store is not self._store:
+            raise ValueError("this AdamW holds the moments of another network: one optimizer per network")
+        self.iterations += 1
+        store.settle()
+        self.batch.step(self.iterations, self.lr, self.beta_1, self.beta_2, self.epsilon, self.weight_decay, grad_scale=grad_scale,
+                        max_norm=self.global_clipnorm, norm=self.grad_norm)
+        store.version += 1
+
+
 class PhiloxSource:
     """Counter-based normal/uniform source: (seed, running counter offset).  Every draw advances the
     offset by the number of Philox blocks it consumed, so a sequence of draws is reproducible."""

@@ -4,7 +4,7 @@ from typing import Callable
 
 import torch
 
-from downscaling.engine.trainer import AdamTF
+from downscaling.engine.trainer import AdamTF, AdamW  # noqa: F401
 from downscaling.gan.metrics import wind_speed_weighted_rmse, discriminator_score_real, discriminator_score_fake  # noqa: F401
 
 generator_losses = [wind_speed_weighted_rmse]
