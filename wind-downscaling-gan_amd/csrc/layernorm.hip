@@ -35,6 +35,244 @@ __device__ __forceinline__ float wdg_ln_block_sum(float v, float* red) {
     return s;
 }
 
+// ---- rows that fit the registers of L lanes (C <= 16384) ------------------------------------------------------------------------
+// L lanes (a power of two; more than 64: L / 64 waves) hold a row, K vectors of V elements each, so x and dz are read once.  A thread's
+// columns are the same for every row it meets: gamma, beta and the parameter sums stay in its registers while the workgroup walks
+// over the rows.
+//
+// The last lanes of a row whose width is not L K V take the row's last V columns again instead of a shorter vector: their first `dup`
+// elements belong to other lanes and count nowhere, what they store there is what the owner stores.  So every request is a whole
+// vector inside the row, whatever the width.
+template <int V, int K, int L>
+struct WdgLnCols {
+    int col[K], dup[K];                                  // first column of vector k; elements j < dup are another lane's
+    __device__ __forceinline__ WdgLnCols(int sub, int C) {
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            const int c0 = (k * L + sub) * V;
+            col[k] = min(c0, C - V);
+            dup[k] = c0 - col[k];
+        }
+    }
+};
+
+// U values summed over the L lanes of each row, results in every lane.  More than one wave per row: through LDS, [U][NT / 64] floats at
+// `red`, one barrier.  The caller gives two calls in a row different places: a wave that is ahead writes the second call's values while
+// another one may still read the first's, and has passed the second's barrier, which that one reaches after reading, before the third.
+template <int L, int NT, int U>
+__device__ __forceinline__ void wdg_ln_row_sums(float (&v)[U], float* red) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        if constexpr (L >= 64) v[u] = wdg_wave_sum_fast(v[u]);
+        else {
+            if constexpr (L >= 2) v[u] = WDG_DPP_ADD(v[u], 0xB1);
+            if constexpr (L >= 4) v[u] = WDG_DPP_ADD(v[u], 0x4E);
+            if constexpr (L >= 8) v[u] = WDG_DPP_ADD(v[u], 0x141);
+            if constexpr (L >= 16) v[u] = WDG_DPP_ADD(v[u], 0x140);
+            if constexpr (L >= 32) v[u] += __shfl_xor(v[u], 16, 64);
+        }
+    }
+    if constexpr (L > 64) {
+        constexpr int W = NT / 64;
+        const int wave = threadIdx.x >> 6;
+        if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) red[u * W + wave] = v[u];
+        }
+        __syncthreads();
+        const int w0 = (threadIdx.x / L) * (L / 64);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            float s = 0.f;
+#pragma unroll
+            for (int w = 0; w < L / 64; ++w) s += red[u * W + w0 + w];
+            v[u] = s;
+        }
+    }
+}
+
+template <class T, int V, int K, int L, int NT, int U, bool TAIL>
+__global__ void __launch_bounds__(NT) wdg_layernorm_fwd_kernel(const T* x, int64_t ldx, const void* __restrict__ gamma,
+                                                               const void* __restrict__ beta, int ptype, float eps, T* z, int64_t ldz,
+                                                               float* mean_rstd, int64_t P, int C) {
+    constexpr int RG = NT / L;                           // rows at a time
+    __shared__ float red[L > 64 ? 3 * U * (NT / 64) : 1];
+    const int sub = threadIdx.x % L, g = threadIdx.x / L;
+    const WdgLnCols<V, K, L> at(sub, C);
+    const float invC = 1.f / (float)C;
+    float gm[K][V], bt[K][V];
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            gm[k][j] = wdg_ln_param<T>(gamma, ptype, at.col[k] + j, 1.f);
+            bt[k][j] = wdg_ln_param<T>(beta, ptype, at.col[k] + j, 0.f);
+        }
+    for (int64_t p0 = (int64_t)blockIdx.x * (RG * U); p0 < P; p0 += (int64_t)gridDim.x * (RG * U)) {
+        WdgVec<T, V> xv[U][K];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t p = std::min<int64_t>(p0 + u * RG + g, P - 1);
+#pragma unroll
+            for (int k = 0; k < K; ++k) xv[u][k] = wdg_vec_load<T, V>(x + p * ldx + at.col[k]);
+        }
+        float s[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            s[u] = 0.f;
+#pragma unroll
+            for (int k = 0; k < K; ++k)
+#pragma unroll
+                for (int j = 0; j < V; ++j) s[u] += TAIL && j < at.dup[k] ? 0.f : (float)xv[u][k].e[j];
+        }
+        wdg_ln_row_sums<L, NT, U>(s, red);
+        float d2[2 * U];                                 // sums of (x - mean) and of its square
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            s[u] *= invC;
+            d2[2 * u] = d2[2 * u + 1] = 0.f;
+#pragma unroll
+            for (int k = 0; k < K; ++k)
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    const float d = TAIL && j < at.dup[k] ? 0.f : (float)xv[u][k].e[j] - s[u];
+                    d2[2 * u] += d;
+                    d2[2 * u + 1] += d * d;
+                }
+        }
+        wdg_ln_row_sums<L, NT, 2 * U>(d2, red + (L > 64 ? U * (NT / 64) : 0));
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t p = p0 + u * RG + g;
+            const float corr = d2[2 * u] * invC;
+            float var = d2[2 * u + 1] * invC - corr * corr;
+            var = var < 0.f ? 0.f : var;                 // (a NaN stays one)
+            const float rstd = 1.f / sqrtf(var + eps);
+            if (p < P) {
+#pragma unroll
+                for (int k = 0; k < K; ++k) {
+                    WdgVec<T, V> r;
+#pragma unroll
+                    for (int j = 0; j < V; ++j) r.e[j] = (T)(((((float)xv[u][k].e[j] - s[u]) - corr) * rstd) * gm[k][j] + bt[k][j]);
+                    if (!TAIL || at.dup[k] < V) wdg_vec_store<T, V>(z + p * ldz + at.col[k], r);
+                }
+                if (mean_rstd && sub == 0) {
+                    mean_rstd[2 * p] = s[u] + corr;
+                    mean_rstd[2 * p + 1] = rstd;
+                }
+            }
+        }
+    }
+}
+
+// part: NULL, or one row [dgamma | dbeta] of partial sums per workgroup
+template <class T, int V, int K, int L, int NT, int U, bool TAIL>
+__global__ void __launch_bounds__(NT) wdg_layernorm_bwd_kernel(const T* dz, int64_t lddz, const T* x, int64_t ldx,
+                                                               const float* __restrict__ mean_rstd, const void* __restrict__ gamma, int ptype,
+                                                               T* dx, int64_t lddx, float* part, int64_t P, int C) {
+    constexpr int RG = NT / L, COPIES = L > 64 ? RG : NT / 64;      // holders of the same columns after the sum within a wave
+    __shared__ float red[L > 64 ? 2 * 2 * U * (NT / 64) : 1];
+    __shared__ float gather[COPIES > 1 ? NT * V : 1];
+    const int t = threadIdx.x, sub = t % L, g = t / L;
+    const WdgLnCols<V, K, L> at(sub, C);
+    const float invC = 1.f / (float)C;
+    float gm[K][V], sg[K][V], sb[K][V];
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            gm[k][j] = wdg_ln_param<T>(gamma, ptype, at.col[k] + j, 1.f);
+            sg[k][j] = sb[k][j] = 0.f;
+        }
+    int turn = 0;
+    for (int64_t p0 = (int64_t)blockIdx.x * (RG * U); p0 < P; p0 += (int64_t)gridDim.x * (RG * U)) {
+        WdgVec<T, V> xv[U][K], gv[U][K];
+        float mean[U], rstd[U], s[2 * U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t p = std::min<int64_t>(p0 + u * RG + g, P - 1);
+            mean[u] = mean_rstd[2 * p];
+            rstd[u] = mean_rstd[2 * p + 1];
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                xv[u][k] = wdg_vec_load<T, V>(x + p * ldx + at.col[k]);
+                gv[u][k] = wdg_vec_load<T, V>(dz + p * lddz + at.col[k]);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const bool on = p0 + u * RG + g < P;
+            s[2 * u] = s[2 * u + 1] = 0.f;
+#pragma unroll
+            for (int k = 0; k < K; ++k)
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    const float gg = (float)gv[u][k].e[j], xh = ((float)xv[u][k].e[j] - mean[u]) * rstd[u], a = gg * gm[k][j];
+                    s[2 * u] += TAIL && j < at.dup[k] ? 0.f : a;
+                    s[2 * u + 1] += TAIL && j < at.dup[k] ? 0.f : a * xh;
+                    if (on) {                            // (elements j < dup gather too, and are left out below)
+                        sg[k][j] += gg * xh;
+                        sb[k][j] += gg;
+                    }
+                }
+        }
+        wdg_ln_row_sums<L, NT, 2 * U>(s, red + (L > 64 ? turn * 2 * U * (NT / 64) : 0));
+        turn ^= 1;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t p = p0 + u * RG + g;
+            const float m1 = s[2 * u] * invC, m2 = s[2 * u + 1] * invC;
+            if (p < P) {
+#pragma unroll
+                for (int k = 0; k < K; ++k) {
+                    WdgVec<T, V> r;
+#pragma unroll
+                    for (int j = 0; j < V; ++j) {
+                        const float xh = ((float)xv[u][k].e[j] - mean[u]) * rstd[u];
+                        r.e[j] = (T)(rstd[u] * ((float)gv[u][k].e[j] * gm[k][j] - m1 - xh * m2));
+                    }
+                    if (!TAIL || at.dup[k] < V) wdg_vec_store<T, V>(dx + p * lddx + at.col[k], r);
+                }
+            }
+        }
+    }
+    if (!part) return;
+    // the workgroup's sums of each column, in a fixed order: lanes of a wave that hold the same columns, then the holders through LDS
+    float* row = part + (int64_t)blockIdx.x * 2 * C;
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int which = 0; which < 2; ++which) {
+            float v[V];
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                v[j] = which ? sb[k][j] : sg[k][j];
+#pragma unroll
+                for (int o = L; o < 64; o <<= 1) v[j] += __shfl_xor(v[j], o, 64);
+            }
+            if constexpr (COPIES > 1) {
+                constexpr int STEP = L > 64 ? L : 64;
+                __syncthreads();
+#pragma unroll
+                for (int j = 0; j < V; ++j) gather[j * NT + t] = v[j];
+                __syncthreads();
+                if (t < L) {
+#pragma unroll
+                    for (int j = 0; j < V; ++j) {
+                        v[j] = 0.f;
+#pragma unroll
+                        for (int w = 0; w < COPIES; ++w) v[j] += gather[j * NT + w * STEP + t];
+                    }
+                }
+            }
+            if (t < L) {
+#pragma unroll
+                for (int j = 0; j < V; ++j)
+                    if (!TAIL || j >= at.dup[k]) row[which * C + at.col[k] + j] = v[j];
+            }
+        }
+}
+
 // ---- any width: one block per row, the row read once per pass -------------------------------------------------------------------
 // The last, partial vector of a row is taken element by element (never beyond the row: what follows may be another row, or nothing).
 constexpr int LNW_NT = 1024;
@@ -212,15 +450,77 @@ __global__ void __launch_bounds__(1024) wdg_layernorm_finish_kernel(const float*
 }
 
 // ---- host side ---------------------------------------------------------------------------------------------------------------------
-struct LnBwdGeom {
-    int slices;          // rows of the partial-sum table
+// How a [P][C] tensor of vectors of V elements is cut: lanes per row, vectors per lane, threads per workgroup, rows in flight per thread.
+// L == 0: the row does not fit (the kernels that read it once per pass take it).
+struct LnGeom {
+    int L, K, NT, U, V;
+    int blocks;                                          // of the register kernels; also the rows of the backward's partial sums
+    int slices;                                          // partial sums of the column kernel (L == 0)
 };
-static LnBwdGeom ln_bwd_geom(int64_t P, int64_t C, int type) {
-    LnBwdGeom g;
-    const int V = type == WDG_F32 ? 4 : 8;
-    const int64_t tiles = (C + 256 * V - 1) / (256 * V);
-    g.slices = (int)std::max<int64_t>(1, std::min<int64_t>((P + 15) / 16, std::max<int64_t>(1, 1024 / tiles)));
+constexpr int LN_CUS = 256;
+
+static LnGeom ln_geom(int64_t P, int64_t C, int type, bool bwd) {
+    LnGeom g = {0, 1, 256, 1, type == WDG_F32 ? 4 : 8, 1, 0};
+    if (C < g.V) {
+        g.V = 1;
+        g.L = 8;
+        g.U = 4;
+    } else {
+        const int64_t vecs = (C + g.V - 1) / g.V;
+        const int most = g.V == 4 ? 4 : 2;               // vectors per lane: 16 elements, so that three fp32 values per column fit
+        if (vecs <= 64) {
+            g.L = 1;
+            while (g.L < vecs) g.L <<= 1;
+            g.U = 4;
+        } else if (vecs <= 64 * most) {
+            g.L = 64;
+            g.K = vecs <= 128 ? 2 : 4;
+            g.U = 4 / g.K;
+        } else if (vecs <= 1024 * most) {
+            g.L = vecs <= 256 * most ? 256 : vecs <= 512 * most ? 512 : 1024;
+            g.K = vecs <= 256 * (most / 2) ? most / 2 : most;
+            g.NT = g.L;
+            g.U = 1;
+        }
+    }
+    if (g.L) {
+        const int64_t rows = (int64_t)(g.NT / g.L) * g.U, resident = (int64_t)LN_CUS * (bwd ? 1024 : 2048) / g.NT;
+        g.blocks = (int)std::max<int64_t>(1, std::min<int64_t>((P + rows - 1) / rows, resident));
+    } else {
+        const int64_t tiles = (C + 256 * g.V - 1) / (256 * g.V);
+        g.slices = (int)std::max<int64_t>(1, std::min<int64_t>((P + 15) / 16, std::max<int64_t>(1, 1024 / tiles)));
+    }
     return g;
+}
+
+// F::template run<V, K, L, NT, U>() for the geometry; false: no register kernel for it
+template <int V, class F>
+static bool ln_dispatch(const LnGeom& g, F&& f) {
+    if (V == 1) {
+        f.template run<1, 1, 8, 256, 4>();
+        return true;
+    }
+    constexpr int M = V == 4 ? 4 : 2;
+    switch (g.L) {
+        case 1: f.template run<V, 1, 1, 256, 4>(); return true;
+        case 2: f.template run<V, 1, 2, 256, 4>(); return true;
+        case 4: f.template run<V, 1, 4, 256, 4>(); return true;
+        case 8: f.template run<V, 1, 8, 256, 4>(); return true;
+        case 16: f.template run<V, 1, 16, 256, 4>(); return true;
+        case 32: f.template run<V, 1, 32, 256, 4>(); return true;
+        case 64:
+            if (g.K == 1) f.template run<V, 1, 64, 256, 4>();
+            else if (g.K == 2) f.template run<V, 2, 64, 256, 2>();
+            else f.template run<V, M, 64, 256, 1>();
+            return true;
+        case 256:
+            if (g.K == M) f.template run<V, M, 256, 256, 1>();
+            else f.template run<V, M / 2, 256, 256, 1>();
+            return true;
+        case 512: f.template run<V, M, 512, 512, 1>(); return true;
+        case 1024: f.template run<V, M, 1024, 1024, 1>(); return true;
+    }
+    return false;
 }
 
 static bool ln_types_ok(int type, int ptype) {
@@ -228,12 +528,36 @@ static bool ln_types_ok(int type, int ptype) {
 }
 static const int64_t LN_MAX_C = 1ll << 24;      // (c / C and the sums' fp32 scale stay exact to rounding)
 
+template <class T>
+struct LnFwd {
+    const T* x;
+    int64_t ldx;
+    const void *gamma, *beta;
+    int ptype;
+    float eps;
+    T* z;
+    int64_t ldz;
+    float* mean_rstd;
+    int64_t P, C;
+    hipStream_t st;
+    LnGeom g;
+    template <int V, int K, int L, int NT, int U>
+    void run() {
+        if (C == (int64_t)V * K * L)
+            hipLaunchKernelGGL((wdg_layernorm_fwd_kernel<T, V, K, L, NT, U, false>), dim3(g.blocks), dim3(NT), 0, st, x, ldx, gamma, beta, ptype, eps, z, ldz, mean_rstd, P, (int)C);
+        else
+            hipLaunchKernelGGL((wdg_layernorm_fwd_kernel<T, V, K, L, NT, U, true>), dim3(g.blocks), dim3(NT), 0, st, x, ldx, gamma, beta, ptype, eps, z, ldz, mean_rstd, P, (int)C);
+    }
+};
+
 template <class T, int V>
 static int ln_fwd_launch(const void* x, int64_t ldx, const void* gamma, const void* beta, int ptype, float eps, void* z, int64_t ldz,
-                         float* mean_rstd, int64_t P, int64_t C, hipStream_t st) {
-    const int blocks = (int)std::min<int64_t>(P, 4096);
-    hipLaunchKernelGGL((wdg_layernorm_fwd_wide_kernel<T, V>), dim3(blocks), dim3(LNW_NT), 0, st, (const T*)x, ldx, gamma, beta, ptype, eps,
-                       (T*)z, ldz, mean_rstd, P, C);
+                         float* mean_rstd, int64_t P, int64_t C, int type, hipStream_t st) {
+    LnFwd<T> f = {(const T*)x, ldx, gamma, beta, ptype, eps, (T*)z, ldz, mean_rstd, P, C, st, ln_geom(P, C, type, false)};
+    if (f.g.V == 1) ln_dispatch<1>(f.g, f);
+    else if (!ln_dispatch<V>(f.g, f))
+        hipLaunchKernelGGL((wdg_layernorm_fwd_wide_kernel<T, V>), dim3((unsigned)std::min<int64_t>(P, 4096)), dim3(LNW_NT), 0, st, (const T*)x, ldx,
+                           gamma, beta, ptype, eps, (T*)z, ldz, mean_rstd, P, C);
     WDG_LAUNCH_CHECK();
     return WDG_OK;
 }
@@ -246,14 +570,15 @@ extern "C" int wdg_layernorm_fwd(const void* x, int64_t ldx, const void* gamma, 
     WDG_CHECK_ARG(x && z, "null argument");
     WDG_CHECK_ARG(ldx >= 0 && (P == 1 || ldz >= C), "output rows overlap");
     hipStream_t st = (hipStream_t)stream;
-    if (type == WDG_F32) return ln_fwd_launch<float, 4>(x, ldx, gamma, beta, param_type, eps, z, ldz, mean_rstd, P, C, st);
-    if (type == WDG_BF16) return ln_fwd_launch<__bf16, 8>(x, ldx, gamma, beta, param_type, eps, z, ldz, mean_rstd, P, C, st);
-    return ln_fwd_launch<_Float16, 8>(x, ldx, gamma, beta, param_type, eps, z, ldz, mean_rstd, P, C, st);
+    if (type == WDG_F32) return ln_fwd_launch<float, 4>(x, ldx, gamma, beta, param_type, eps, z, ldz, mean_rstd, P, C, type, st);
+    if (type == WDG_BF16) return ln_fwd_launch<__bf16, 8>(x, ldx, gamma, beta, param_type, eps, z, ldz, mean_rstd, P, C, type, st);
+    return ln_fwd_launch<_Float16, 8>(x, ldx, gamma, beta, param_type, eps, z, ldz, mean_rstd, P, C, type, st);
 }
 
 extern "C" size_t wdg_layernorm_bwd_ws_bytes(int64_t P, int64_t C, int type) {
     if (P <= 0 || C <= 0 || C > LN_MAX_C || type < WDG_F32 || type > WDG_F16) return 0;
-    return (size_t)ln_bwd_geom(P, C, type).slices * 2 * (size_t)C * sizeof(float);
+    const LnGeom g = ln_geom(P, C, type, true);
+    return (size_t)(g.L ? g.blocks : g.slices) * 2 * (size_t)C * sizeof(float);
 }
 
 static int ln_finish(const float* part, int rows, int64_t C, float* dgamma, float* dbeta, int accumulate, hipStream_t st) {
@@ -265,25 +590,51 @@ static int ln_finish(const float* part, int rows, int64_t C, float* dgamma, floa
     return WDG_OK;
 }
 
+template <class T>
+struct LnBwd {
+    const T* dz;
+    int64_t lddz;
+    const T* x;
+    int64_t ldx;
+    const float* mean_rstd;
+    const void* gamma;
+    int ptype;
+    T* dx;
+    int64_t lddx;
+    float* part;
+    int64_t P, C;
+    hipStream_t st;
+    LnGeom g;
+    template <int V, int K, int L, int NT, int U>
+    void run() {
+        if (C == (int64_t)V * K * L)
+            hipLaunchKernelGGL((wdg_layernorm_bwd_kernel<T, V, K, L, NT, U, false>), dim3(g.blocks), dim3(NT), 0, st, dz, lddz, x, ldx, mean_rstd, gamma, ptype, dx, lddx, part, P, (int)C);
+        else
+            hipLaunchKernelGGL((wdg_layernorm_bwd_kernel<T, V, K, L, NT, U, true>), dim3(g.blocks), dim3(NT), 0, st, dz, lddz, x, ldx, mean_rstd, gamma, ptype, dx, lddx, part, P, (int)C);
+    }
+};
+
 template <class T, int V>
 static int ln_bwd_launch(const void* dz, int64_t lddz, const void* x, int64_t ldx, const float* mean_rstd, const void* gamma, int ptype,
                          void* dx, int64_t lddx, float* dgamma, float* dbeta, int accumulate, int64_t P, int64_t C, int type, float* part,
                          hipStream_t st) {
-    if (dgamma || dbeta) {
-        const int slices = P > 0 ? ln_bwd_geom(P, C, type).slices : 0;
-        if (slices > 0) {
-            hipLaunchKernelGGL((wdg_layernorm_colsum_kernel<T, V>), dim3((unsigned)((C + 256 * V - 1) / (256 * V)), slices), dim3(256), 0, st,
-                               (const T*)dz, lddz, (const T*)x, ldx, mean_rstd, part, P, C, slices);
+    const bool params = dgamma || dbeta;
+    if (P == 0) return params ? ln_finish(part, 0, C, dgamma, dbeta, accumulate, st) : WDG_OK;
+    LnBwd<T> f = {(const T*)dz, lddz, (const T*)x, ldx, mean_rstd, gamma, ptype, (T*)dx, lddx, params ? part : nullptr, P, C, st, ln_geom(P, C, type, true)};
+    int rows = f.g.blocks;
+    if (f.g.V == 1) ln_dispatch<1>(f.g, f);
+    else if (!ln_dispatch<V>(f.g, f)) {
+        if (params) {
+            rows = f.g.slices;
+            hipLaunchKernelGGL((wdg_layernorm_colsum_kernel<T, V>), dim3((unsigned)((C + 256 * V - 1) / (256 * V)), rows), dim3(256), 0, st,
+                               (const T*)dz, lddz, (const T*)x, ldx, mean_rstd, part, P, C, rows);
             WDG_LAUNCH_CHECK();
         }
-        const int rc = ln_finish(part, slices, C, dgamma, dbeta, accumulate, st);
-        if (rc != WDG_OK) return rc;
+        hipLaunchKernelGGL((wdg_layernorm_bwd_wide_kernel<T, V>), dim3((unsigned)std::min<int64_t>(P, 4096)), dim3(LNW_NT), 0, st, (const T*)dz,
+                           lddz, (const T*)x, ldx, mean_rstd, gamma, ptype, (T*)dx, lddx, P, C);
     }
-    if (P == 0) return WDG_OK;
-    hipLaunchKernelGGL((wdg_layernorm_bwd_wide_kernel<T, V>), dim3((unsigned)std::min<int64_t>(P, 4096)), dim3(LNW_NT), 0, st, (const T*)dz,
-                       lddz, (const T*)x, ldx, mean_rstd, gamma, ptype, (T*)dx, lddx, P, C);
     WDG_LAUNCH_CHECK();
-    return WDG_OK;
+    return params ? ln_finish(part, rows, C, dgamma, dbeta, accumulate, st) : WDG_OK;
 }
 
 extern "C" int wdg_layernorm_bwd(const void* dz, int64_t lddz, const void* x, int64_t ldx, const float* mean_rstd, const void* gamma,
