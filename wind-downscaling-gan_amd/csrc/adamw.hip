@@ -13,7 +13,7 @@
 
 constexpr int AW_CHUNK = 4096;     // elements per record
 constexpr int AW_BLOCK = 256;      // elements that share a scale of the 8-bit states
-constexpr int AW_PARTS = 256;      // partial sums of the gradient norm
+constexpr int AW_PARTS = 512;      // partial sums of the gradient norm
 
 struct WdgAdamwChunk {
     void* p;
@@ -76,11 +76,14 @@ __device__ __forceinline__ void wdg_aw_store(T* p, int n, const f32x4& r) {
     }
 }
 
-// largest of 64 lanes' unsigned values, in every lane
+// largest of 64 lanes' unsigned values, in every lane: within rows of 16 lanes by DPP, the four rows through scalar registers
 __device__ __forceinline__ unsigned wdg_wave_umax(unsigned v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v = max(v, (unsigned)__shfl_xor((int)v, o, 64));
-    return v;
+    v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xF, 0xF, true));     // quad_perm [1,0,3,2]
+    v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xF, 0xF, true));     // quad_perm [2,3,0,1]
+    v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x141, 0xF, 0xF, true));    // row_half_mirror
+    v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x140, 0xF, 0xF, true));    // row_mirror
+    return max(max((unsigned)__builtin_amdgcn_readlane((int)v, 0), (unsigned)__builtin_amdgcn_readlane((int)v, 16)),
+               max((unsigned)__builtin_amdgcn_readlane((int)v, 32), (unsigned)__builtin_amdgcn_readlane((int)v, 48)));
 }
 // A block's scale from the largest bit pattern of its magnitudes (as integers: above infinity come the NaNs, which a float maximum would
 // drop).  inv = 1 / scale, 0 where the block holds zeros alone; a block that is not finite gets a NaN for its scale.
@@ -115,84 +118,102 @@ __device__ __forceinline__ bool wdg_aw_clip(const WdgAdamwHyper& h, double* red,
     return true;
 }
 
-template <int BITS, class PT, class GT>
+// One chunk.  FULL: all 4096 elements are there, so every request is issued without a condition, those of UN quads per thread before
+// the first of them is used; else the tensor ends inside, and each quad looks at what is left.
+template <int BITS, class PT, class GT, bool FULL>
 __device__ __forceinline__ void wdg_aw_chunk(const WdgAdamwChunk& q, const WdgAdamwHyper& h, float gs, float lr_bc1, float rbc2) {
+    constexpr int UN = !FULL ? 1 : BITS == 32 ? 2 : 4;
     const float keep = 1.f - h.lr_wd * q.decay;
     PT* p = static_cast<PT*>(q.p);
     const GT* g = static_cast<const GT*>(q.g);
     const int lane = threadIdx.x & 63;
 #pragma unroll 1
-    for (int i = 0; i < AW_CHUNK / 1024; ++i) {
-        const int e = (i * 256 + (int)threadIdx.x) * 4;
-        if (i * 1024 + ((int)threadIdx.x & ~63) * 4 >= q.n) break;        // (the wave's whole block lies behind the tensor)
-        const int n = q.n - e;                                           // elements from here on; may be negative for the last lanes
-        f32x4 w = wdg_aw_load(p + e, n);
-        const f32x4 gr = wdg_aw_load(g + e, n);
-        f32x4 m, v;
-        if constexpr (BITS == 32) {
-            m = wdg_aw_load(static_cast<const float*>(q.m) + e, n);
-            v = wdg_aw_load(static_cast<const float*>(q.v) + e, n);
-        } else {
-            const unsigned cm = static_cast<const unsigned*>(q.m)[e >> 2], cv = static_cast<const unsigned*>(q.v)[e >> 2];
-            const float sm = q.ms[e / AW_BLOCK] * (1.f / (127.f * 127.f)), sv = q.vs[e / AW_BLOCK];
+    for (int i = 0; i < AW_CHUNK / 1024; i += UN) {
+        if (!FULL && i * 1024 + ((int)threadIdx.x & ~63) * 4 >= q.n) break;       // (the wave's whole block lies behind the tensor)
+        f32x4 w[UN], gr[UN], m[UN], v[UN];
+        unsigned cm[UN], cv[UN];
+        float sm[UN], sv[UN];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const float a = (float)(signed char)(cm >> (8 * j)), b = (float)((cv >> (8 * j)) & 255u) * (1.f / 255.f);
-                m[j] = a * fabsf(a) * sm;
-                v[j] = (b * b) * (b * b) * sv;
+        for (int k = 0; k < UN; ++k) {
+            const int e = ((i + k) * 256 + (int)threadIdx.x) * 4, n = FULL ? 4 : q.n - e;      // (n: elements from here on, maybe none)
+            w[k] = wdg_aw_load(p + e, n);
+            gr[k] = wdg_aw_load(g + e, n);
+            if constexpr (BITS == 32) {
+                m[k] = wdg_aw_load(static_cast<const float*>(q.m) + e, n);
+                v[k] = wdg_aw_load(static_cast<const float*>(q.v) + e, n);
+            } else {
+                cm[k] = static_cast<const unsigned*>(q.m)[e >> 2];
+                cv[k] = static_cast<const unsigned*>(q.v)[e >> 2];
+                sm[k] = q.ms[e / AW_BLOCK];
+                sv[k] = q.vs[e / AW_BLOCK];
             }
         }
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float gj = gr[j] * gs;
-            m[j] = h.b1 * m[j] + h.c1 * gj;
-            v[j] = h.b2 * v[j] + h.c2 * (gj * gj);
-            w[j] = w[j] * keep - lr_bc1 * (m[j] / (sqrtf(v[j]) * rbc2 + h.eps));
-        }
-        wdg_aw_store(p + e, n, w);
-        if (q.copy_type == WDG_BF16) wdg_aw_store(static_cast<__bf16*>(q.copy) + e, n, w);
-        else if (q.copy_type == WDG_F16) wdg_aw_store(static_cast<_Float16*>(q.copy) + e, n, w);
-        if constexpr (BITS == 32) {
-            wdg_aw_store(static_cast<float*>(q.m) + e, n, m);
-            wdg_aw_store(static_cast<float*>(q.v) + e, n, v);
-        } else {
+        for (int k = 0; k < UN; ++k) {
+            const int e = ((i + k) * 256 + (int)threadIdx.x) * 4, n = FULL ? 4 : q.n - e;
+            if constexpr (BITS == 8) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float a = (float)(signed char)(cm[k] >> (8 * j)), b = (float)((cv[k] >> (8 * j)) & 255u) * (1.f / 255.f);
+                    m[k][j] = a * fabsf(a) * (sm[k] * (1.f / (127.f * 127.f)));
+                    v[k][j] = (b * b) * (b * b) * sv[k];
+                }
+            }
             unsigned tm = 0, tv = 0;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const float a = m[j], b = v[j];           // (a bit cast of a vector's element would take element 0)
-                tm = max(tm, j < n ? __builtin_bit_cast(unsigned, a) & 0x7fffffffu : 0u);
-                tv = max(tv, j < n ? __builtin_bit_cast(unsigned, b) & 0x7fffffffu : 0u);
+                const float gj = gr[k][j] * gs;
+                const float a = h.b1 * m[k][j] + h.c1 * gj, b = h.b2 * v[k][j] + h.c2 * (gj * gj);
+                m[k][j] = a;
+                v[k][j] = b;
+                w[k][j] = w[k][j] * keep - lr_bc1 * (a / (sqrtf(b) * rbc2 + h.eps));
+                if constexpr (BITS == 8) {               // (from the scalars: a bit cast of a vector's element would take element 0)
+                    tm = max(tm, j < n ? __builtin_bit_cast(unsigned, a) & 0x7fffffffu : 0u);
+                    tv = max(tv, j < n ? __builtin_bit_cast(unsigned, b) & 0x7fffffffu : 0u);
+                }
             }
-            float im, iv;
-            const float sm = wdg_aw_scale(wdg_wave_umax(tm), im), sv = wdg_aw_scale(wdg_wave_umax(tv), iv);
-            unsigned cm = 0, cv = 0;
+            wdg_aw_store(p + e, n, w[k]);
+            if (q.copy_type == WDG_BF16) wdg_aw_store(static_cast<__bf16*>(q.copy) + e, n, w[k]);
+            else if (q.copy_type == WDG_F16) wdg_aw_store(static_cast<_Float16*>(q.copy) + e, n, w[k]);
+            if constexpr (BITS == 32) {
+                wdg_aw_store(static_cast<float*>(q.m) + e, n, m[k]);
+                wdg_aw_store(static_cast<float*>(q.v) + e, n, v[k]);
+            } else {
+                float im, iv;
+                const float nm = wdg_aw_scale(wdg_wave_umax(tm), im), nv = wdg_aw_scale(wdg_wave_umax(tv), iv);
+                unsigned om = 0, ov = 0;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                if (j >= n) continue;
-                // both companding roots on the hardware square root (one unit in the last place of a value that is rounded to 1 / 127
-                // or 1 / 255): only a value that close to the border between two codes can take the other one
-                const float a = rintf(127.f * __builtin_amdgcn_sqrtf(fabsf(m[j]) * im));
-                float b = rintf(255.f * __builtin_amdgcn_sqrtf(__builtin_amdgcn_sqrtf(v[j] * iv)));
-                b = v[j] * iv > 0.f ? fmaxf(b, 1.f) : 0.f;
-                const int ai = im > 0.f ? (int)(m[j] < 0.f ? -a : a) : 0, bi = iv > 0.f ? (int)b : 0;
-                cm |= ((unsigned)ai & 255u) << (8 * j);
-                cv |= ((unsigned)bi & 255u) << (8 * j);
-            }
-            static_cast<unsigned*>(q.m)[e >> 2] = cm;
-            static_cast<unsigned*>(q.v)[e >> 2] = cv;
-            if (lane == 0) {
-                q.ms[e / AW_BLOCK] = sm;
-                q.vs[e / AW_BLOCK] = sv;
+                for (int j = 0; j < 4; ++j) {
+                    if (j >= n) continue;
+                    // both companding roots on the hardware square root (one unit in the last place of a value that is rounded to
+                    // 1 / 127 or 1 / 255): only a value that close to the border between two codes can take the other one
+                    const float a = rintf(127.f * __builtin_amdgcn_sqrtf(fabsf(m[k][j]) * im)), r = v[k][j] * iv;
+                    const float b = r > 0.f ? fmaxf(rintf(255.f * __builtin_amdgcn_sqrtf(__builtin_amdgcn_sqrtf(r))), 1.f) : 0.f;
+                    const int ai = im > 0.f ? (int)(m[k][j] < 0.f ? -a : a) : 0, bi = iv > 0.f ? (int)b : 0;
+                    om |= ((unsigned)ai & 255u) << (8 * j);
+                    ov |= ((unsigned)bi & 255u) << (8 * j);
+                }
+                static_cast<unsigned*>(q.m)[e >> 2] = om;
+                static_cast<unsigned*>(q.v)[e >> 2] = ov;
+                if (lane == 0) {
+                    q.ms[e / AW_BLOCK] = nm;
+                    q.vs[e / AW_BLOCK] = nv;
+                }
             }
         }
     }
 }
 
+template <int BITS, class PT, class GT>
+__device__ __forceinline__ void wdg_aw_by_size(const WdgAdamwChunk& q, const WdgAdamwHyper& h, float gs, float lr_bc1, float rbc2) {
+    if (q.n == AW_CHUNK) wdg_aw_chunk<BITS, PT, GT, true>(q, h, gs, lr_bc1, rbc2);
+    else wdg_aw_chunk<BITS, PT, GT, false>(q, h, gs, lr_bc1, rbc2);
+}
 template <int BITS, class PT>
 __device__ __forceinline__ void wdg_aw_by_grad(const WdgAdamwChunk& q, const WdgAdamwHyper& h, float gs, float lr_bc1, float rbc2) {
-    if (q.g_type == WDG_F32) wdg_aw_chunk<BITS, PT, float>(q, h, gs, lr_bc1, rbc2);
-    else if (q.g_type == WDG_BF16) wdg_aw_chunk<BITS, PT, __bf16>(q, h, gs, lr_bc1, rbc2);
-    else wdg_aw_chunk<BITS, PT, _Float16>(q, h, gs, lr_bc1, rbc2);
+    if (q.g_type == WDG_F32) wdg_aw_by_size<BITS, PT, float>(q, h, gs, lr_bc1, rbc2);
+    else if (q.g_type == WDG_BF16) wdg_aw_by_size<BITS, PT, __bf16>(q, h, gs, lr_bc1, rbc2);
+    else wdg_aw_by_size<BITS, PT, _Float16>(q, h, gs, lr_bc1, rbc2);
 }
 
 template <int BITS>
@@ -212,31 +233,47 @@ __global__ void __launch_bounds__(256) wdg_adamw_kernel(const WdgAdamwChunk* __r
     else wdg_aw_by_grad<BITS, _Float16>(q, h, gs, lr_bc1, rbc2);
 }
 
-// ---- sum of g^2 over all chunks: AW_PARTS workgroups, each every AW_PARTS-th chunk; fp64, since a square leaves fp32's range where the
-// gradient itself does not -----------------------------------------------------------------------------------------------------------
+// ---- sum of g^2 over all chunks; fp64, since a square leaves fp32's range where the gradient itself does not -------------------------
+// Four chunks at a time per workgroup (256 threads each), as many workgroups as the chip holds: the launch reads one tensor, and what it
+// needs is requests in flight.
 template <class GT>
 __device__ __forceinline__ double wdg_aw_sumsq(const GT* g, int n) {
-    double s = 0.0;
-    for (int e = (int)threadIdx.x * 4; e < n; e += 1024) {
-        const f32x4 v = wdg_aw_load(g + e, n - e);
+    const int t = (int)(threadIdx.x & 255) * 4;
+    f32x4 v[AW_CHUNK / 1024];
+    if (n == AW_CHUNK) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) s += (double)v[j] * (double)v[j];
+        for (int i = 0; i < AW_CHUNK / 1024; ++i) v[i] = wdg_aw_load(g + i * 1024 + t, 4);
+    } else {
+#pragma unroll
+        for (int i = 0; i < AW_CHUNK / 1024; ++i) v[i] = wdg_aw_load(g + i * 1024 + t, n - i * 1024 - t);
     }
+    double s = 0.0;
+#pragma unroll
+    for (int i = 0; i < AW_CHUNK / 1024; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s += (double)v[i][j] * (double)v[i][j];
     return s;
 }
-__global__ void __launch_bounds__(256) wdg_adamw_sumsq_kernel(const WdgAdamwChunk* __restrict__ table, int chunks, double* parts) {
-    __shared__ double red[4];
+__global__ void __launch_bounds__(1024) wdg_adamw_sumsq_kernel(const WdgAdamwChunk* __restrict__ table, int chunks, double* parts) {
+    __shared__ double red[16];
     double s = 0.0;
-    for (int c = blockIdx.x; c < chunks; c += gridDim.x) {
-        const WdgAdamwChunk q = table[c];
-        if (q.g_type == WDG_F32) s += wdg_aw_sumsq(static_cast<const float*>(q.g), q.n);
-        else if (q.g_type == WDG_BF16) s += wdg_aw_sumsq(static_cast<const __bf16*>(q.g), q.n);
-        else s += wdg_aw_sumsq(static_cast<const _Float16*>(q.g), q.n);
+    for (int c = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 8); c < chunks; c += gridDim.x * 4) {
+        const void* g = table[c].g;
+        const int n = table[c].n;
+        const unsigned char type = table[c].g_type;
+        if (type == WDG_F32) s += wdg_aw_sumsq(static_cast<const float*>(g), n);
+        else if (type == WDG_BF16) s += wdg_aw_sumsq(static_cast<const __bf16*>(g), n);
+        else s += wdg_aw_sumsq(static_cast<const _Float16*>(g), n);
     }
     s = wdg_wave_sum_d(s);
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
     __syncthreads();
-    if (threadIdx.x == 0) parts[blockIdx.x] = (red[0] + red[1]) + (red[2] + red[3]);
+    if (threadIdx.x == 0) {
+        double total = 0.0;
+#pragma unroll
+        for (int w = 0; w < 16; ++w) total += red[w];
+        parts[blockIdx.x] = total;
+    }
 }
 __global__ void __launch_bounds__(256) wdg_adamw_norm_kernel(const double* __restrict__ parts, int nparts, double scale, float* norm) {
     __shared__ double red[4];
@@ -248,24 +285,27 @@ __global__ void __launch_bounds__(256) wdg_adamw_norm_kernel(const double* __res
     if (threadIdx.x == 0) norm[0] = (float)(scale * sqrt((red[0] + red[1]) + (red[2] + red[3])));
 }
 
-// ---- the values behind 8-bit states: four codes per thread, blockIdx.y 0 the first moment, 1 the second ----------------------------
+// ---- the values behind 8-bit states: 16 codes per thread, blockIdx.y 0 the first moment, 1 the second ----------------------------
 template <class T>
-__global__ void __launch_bounds__(256) wdg_adamw_moments_kernel(const unsigned* m, const float* ms, const unsigned* v, const float* vs, T* mo,
-                                                                T* vo, long long quads) {
+__global__ void __launch_bounds__(256) wdg_adamw_moments_kernel(const unsigned char* m, const float* ms, const unsigned char* v, const float* vs,
+                                                                T* mo, T* vo, long long sixteens) {
     const bool second = blockIdx.y == 1;
     T* out = second ? vo : mo;
     if (!out) return;
-    const unsigned* codes = second ? v : m;
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < quads; i += (long long)gridDim.x * 256) {
-        const unsigned c = codes[i];
-        const float s = (second ? vs : ms)[i / (AW_BLOCK / 4)];
-        f32x4 r;
+    const unsigned char* codes = second ? v : m;
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < sixteens; i += (long long)gridDim.x * 256) {
+        const WdgVec<unsigned, 4> c = wdg_vec_load<unsigned, 4>(reinterpret_cast<const unsigned*>(codes) + 4 * i);
+        const float s = (second ? vs : ms)[i / (AW_BLOCK / 16)];
+        const float s1 = s * (1.f / (127.f * 127.f));
+        WdgVec<T, 16> r;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float a = (float)(signed char)(c >> (8 * j)), b = (float)((c >> (8 * j)) & 255u) * (1.f / 255.f);
-            r[j] = second ? (b * b) * (b * b) * s : a * fabsf(a) * (s * (1.f / (127.f * 127.f)));
-        }
-        wdg_aw_store(out + 4 * i, 4, r);
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float a = (float)(signed char)(c.e[k] >> (8 * j)), b = (float)((c.e[k] >> (8 * j)) & 255u) * (1.f / 255.f);
+                r.e[4 * k + j] = (T)(second ? (b * b) * (b * b) * s : a * fabsf(a) * s1);
+            }
+        wdg_vec_store<T, 16>(out + 16 * i, r);
     }
 }
 
@@ -394,11 +434,11 @@ extern "C" int wdg_adamw_destroy(wdg_adamw_batch* b) {
 
 extern "C" size_t wdg_adamw_scratch_bytes(void) { return AW_PARTS * sizeof(double); }
 
-static int aw_parts(const wdg_adamw_batch* b) { return (int)std::min<size_t>(AW_PARTS, b->chunks.size()); }
+static int aw_parts(const wdg_adamw_batch* b) { return (int)std::min<size_t>(AW_PARTS, (b->chunks.size() + 3) / 4); }
 
 static int aw_sumsq(const wdg_adamw_batch* b, double* parts, hipStream_t st) {
     if (aw_parts(b) == 0) return WDG_OK;
-    hipLaunchKernelGGL(wdg_adamw_sumsq_kernel, dim3(aw_parts(b)), dim3(256), 0, st, b->table, (int)b->chunks.size(), parts);
+    hipLaunchKernelGGL(wdg_adamw_sumsq_kernel, dim3(aw_parts(b)), dim3(1024), 0, st, b->table, (int)b->chunks.size(), parts);
     WDG_LAUNCH_CHECK();
     return WDG_OK;
 }
@@ -477,13 +517,13 @@ extern "C" int wdg_adamw_moments(const void* m, const float* m_scale, const void
     if (blocks == 0 || (!m_out && !v_out)) return WDG_OK;
     WDG_CHECK_ARG((!m_out || (m && m_scale)) && (!v_out || (v && v_scale)), "null argument");
     WDG_CHECK_ARG(aw_aligned(m, 4) && aw_aligned(v, 4) && aw_aligned(m_out, aw_bytes(out_type)) && aw_aligned(v_out, aw_bytes(out_type)), "alignment");
-    const long long quads = blocks * (AW_BLOCK / 4);
-    const dim3 grid((unsigned)std::min<long long>((quads + 255) / 256, 8192), 2);
+    const long long sixteens = blocks * (AW_BLOCK / 16);
+    const dim3 grid((unsigned)std::min<long long>((sixteens + 255) / 256, 16384), 2);
     hipStream_t st = (hipStream_t)stream;
-    const unsigned *mc = (const unsigned*)m, *vc = (const unsigned*)v;
-    if (out_type == WDG_F32) hipLaunchKernelGGL(wdg_adamw_moments_kernel<float>, grid, dim3(256), 0, st, mc, m_scale, vc, v_scale, (float*)m_out, (float*)v_out, quads);
-    else if (out_type == WDG_BF16) hipLaunchKernelGGL(wdg_adamw_moments_kernel<__bf16>, grid, dim3(256), 0, st, mc, m_scale, vc, v_scale, (__bf16*)m_out, (__bf16*)v_out, quads);
-    else hipLaunchKernelGGL(wdg_adamw_moments_kernel<_Float16>, grid, dim3(256), 0, st, mc, m_scale, vc, v_scale, (_Float16*)m_out, (_Float16*)v_out, quads);
+    const unsigned char *mc = (const unsigned char*)m, *vc = (const unsigned char*)v;
+    if (out_type == WDG_F32) hipLaunchKernelGGL(wdg_adamw_moments_kernel<float>, grid, dim3(256), 0, st, mc, m_scale, vc, v_scale, (float*)m_out, (float*)v_out, sixteens);
+    else if (out_type == WDG_BF16) hipLaunchKernelGGL(wdg_adamw_moments_kernel<__bf16>, grid, dim3(256), 0, st, mc, m_scale, vc, v_scale, (__bf16*)m_out, (__bf16*)v_out, sixteens);
+    else hipLaunchKernelGGL(wdg_adamw_moments_kernel<_Float16>, grid, dim3(256), 0, st, mc, m_scale, vc, v_scale, (_Float16*)m_out, (_Float16*)v_out, sixteens);
     WDG_LAUNCH_CHECK();
     return WDG_OK;
 }

@@ -108,14 +108,24 @@ __global__ void __launch_bounds__(NT) wdg_layernorm_fwd_kernel(const T* x, int64
             gm[k][j] = wdg_ln_param<T>(gamma, ptype, at.col[k] + j, 1.f);
             bt[k][j] = wdg_ln_param<T>(beta, ptype, at.col[k] + j, 0.f);
         }
-    for (int64_t p0 = (int64_t)blockIdx.x * (RG * U); p0 < P; p0 += (int64_t)gridDim.x * (RG * U)) {
-        WdgVec<T, V> xv[U][K];
+    const int64_t stride = (int64_t)gridDim.x * (RG * U);
+    WdgVec<T, V> ahead[U][K];                            // the next rows are on their way while these are summed (behind the last: again the last)
+    auto fetch = [&](int64_t p0) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int64_t p = std::min<int64_t>(p0 + u * RG + g, P - 1);
 #pragma unroll
-            for (int k = 0; k < K; ++k) xv[u][k] = wdg_vec_load<T, V>(x + p * ldx + at.col[k]);
+            for (int k = 0; k < K; ++k) ahead[u][k] = wdg_vec_load<T, V>(x + p * ldx + at.col[k]);
         }
+    };
+    fetch((int64_t)blockIdx.x * (RG * U));
+    for (int64_t p0 = (int64_t)blockIdx.x * (RG * U); p0 < P; p0 += stride) {
+        WdgVec<T, V> xv[U][K];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int k = 0; k < K; ++k) xv[u][k] = ahead[u][k];
+        fetch(p0 + stride);
         float s[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
