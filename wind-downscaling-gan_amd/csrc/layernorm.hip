@@ -22,6 +22,23 @@ __device__ __forceinline__ float wdg_ln_param(const void* p, int ptype, int64_t 
     return ptype == 0 ? static_cast<const float*>(p)[c] : (float)static_cast<const T*>(p)[c];
 }
 
+// ... V adjacent parameters in one or two requests
+template <class T, int V>
+__device__ __forceinline__ void wdg_ln_params(float (&r)[V], const void* p, int ptype, int64_t c, float none) {
+    if (!p) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) r[j] = none;
+    } else if (ptype == 0) {
+        const WdgVec<float, V> v = wdg_vec_load<float, V>(static_cast<const float*>(p) + c);
+#pragma unroll
+        for (int j = 0; j < V; ++j) r[j] = v.e[j];
+    } else {
+        const WdgVec<T, V> v = wdg_vec_load<T, V>(static_cast<const T*>(p) + c);
+#pragma unroll
+        for (int j = 0; j < V; ++j) r[j] = (float)v.e[j];
+    }
+}
+
 // sum over the block's threads, result in every thread; `red` holds one float per wave, and may be reused after the next barrier
 template <int NT>
 __device__ __forceinline__ float wdg_ln_block_sum(float v, float* red) {
@@ -36,34 +53,34 @@ __device__ __forceinline__ float wdg_ln_block_sum(float v, float* red) {
 }
 
 // ---- rows that fit the registers of L lanes (C <= 16384) ------------------------------------------------------------------------
-// L lanes (a power of two; more than 64: L / 64 waves) hold a row, K vectors of V elements each, so x and dz are read once.  A thread's
+// L lanes (1 .. 64, a power of two; L == 0: all waves of the workgroup) hold a row, K vectors of V elements each, so x and dz are read once.  A thread's
 // columns are the same for every row it meets: gamma, beta and the parameter sums stay in its registers while the workgroup walks
 // over the rows.
 //
 // The last lanes of a row whose width is not L K V take the row's last V columns again instead of a shorter vector: their first `dup`
 // elements belong to other lanes and count nowhere, what they store there is what the owner stores.  So every request is a whole
 // vector inside the row, whatever the width.
-template <int V, int K, int L>
+template <int V, int K>
 struct WdgLnCols {
     int col[K], dup[K];                                  // first column of vector k; elements j < dup are another lane's
-    __device__ __forceinline__ WdgLnCols(int sub, int C) {
+    __device__ __forceinline__ WdgLnCols(int lanes, int sub, int C) {
 #pragma unroll
         for (int k = 0; k < K; ++k) {
-            const int c0 = (k * L + sub) * V;
+            const int c0 = (k * lanes + sub) * V;
             col[k] = min(c0, C - V);
             dup[k] = c0 - col[k];
         }
     }
 };
 
-// U values summed over the L lanes of each row, results in every lane.  More than one wave per row: through LDS, [U][NT / 64] floats at
+// U values summed over the lanes of each row, results in every lane.  A row of the whole workgroup goes through LDS, [U][16] floats at
 // `red`, one barrier.  The caller gives two calls in a row different places: a wave that is ahead writes the second call's values while
 // another one may still read the first's, and has passed the second's barrier, which that one reaches after reading, before the third.
-template <int L, int NT, int U>
+template <int L, int U>
 __device__ __forceinline__ void wdg_ln_row_sums(float (&v)[U], float* red) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-        if constexpr (L >= 64) v[u] = wdg_wave_sum_fast(v[u]);
+        if constexpr (L == 0 || L == 64) v[u] = wdg_wave_sum_fast(v[u]);
         else {
             if constexpr (L >= 2) v[u] = WDG_DPP_ADD(v[u], 0xB1);
             if constexpr (L >= 4) v[u] = WDG_DPP_ADD(v[u], 0x4E);
@@ -72,22 +89,16 @@ __device__ __forceinline__ void wdg_ln_row_sums(float (&v)[U], float* red) {
             if constexpr (L >= 32) v[u] += __shfl_xor(v[u], 16, 64);
         }
     }
-    if constexpr (L > 64) {
-        constexpr int W = NT / 64;
-        const int wave = threadIdx.x >> 6;
+    if constexpr (L == 0) {
         if ((threadIdx.x & 63) == 0) {
 #pragma unroll
-            for (int u = 0; u < U; ++u) red[u * W + wave] = v[u];
+            for (int u = 0; u < U; ++u) red[u * 16 + (threadIdx.x >> 6)] = v[u];
         }
         __syncthreads();
-        const int w0 = (threadIdx.x / L) * (L / 64);
+        // every lane takes one wave's value (lanes 0 .. 15 of each row of 16), the row sum adds them
+        const int w = threadIdx.x & 15, waves = blockDim.x >> 6;
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            float s = 0.f;
-#pragma unroll
-            for (int w = 0; w < L / 64; ++w) s += red[u * W + w0 + w];
-            v[u] = s;
-        }
+        for (int u = 0; u < U; ++u) v[u] = wdg_row16_sum(w < waves ? red[u * 16 + w] : 0.f);
     }
 }
 
@@ -95,19 +106,17 @@ template <class T, int V, int K, int L, int NT, int U, bool TAIL>
 __global__ void __launch_bounds__(NT) wdg_layernorm_fwd_kernel(const T* x, int64_t ldx, const void* __restrict__ gamma,
                                                                const void* __restrict__ beta, int ptype, float eps, T* z, int64_t ldz,
                                                                float* mean_rstd, int64_t P, int C) {
-    constexpr int RG = NT / L;                           // rows at a time
-    __shared__ float red[L > 64 ? 3 * U * (NT / 64) : 1];
-    const int sub = threadIdx.x % L, g = threadIdx.x / L;
-    const WdgLnCols<V, K, L> at(sub, C);
+    constexpr int RG = L ? NT / (L ? L : 1) : 1;         // rows at a time
+    __shared__ float red[L ? 1 : 3 * U * 16];
+    const int lanes = L ? L : blockDim.x, sub = threadIdx.x % lanes, g = threadIdx.x / lanes;
+    const WdgLnCols<V, K> at(lanes, sub, C);
     const float invC = 1.f / (float)C;
     float gm[K][V], bt[K][V];
 #pragma unroll
-    for (int k = 0; k < K; ++k)
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-            gm[k][j] = wdg_ln_param<T>(gamma, ptype, at.col[k] + j, 1.f);
-            bt[k][j] = wdg_ln_param<T>(beta, ptype, at.col[k] + j, 0.f);
-        }
+    for (int k = 0; k < K; ++k) {
+        wdg_ln_params<T, V>(gm[k], gamma, ptype, at.col[k], 1.f);
+        wdg_ln_params<T, V>(bt[k], beta, ptype, at.col[k], 0.f);
+    }
     const int64_t stride = (int64_t)gridDim.x * (RG * U);
     WdgVec<T, V> ahead[U][K];                            // the next rows are on their way while these are summed (behind the last: again the last)
     auto fetch = [&](int64_t p0) {
@@ -135,7 +144,7 @@ __global__ void __launch_bounds__(NT) wdg_layernorm_fwd_kernel(const T* x, int64
 #pragma unroll
                 for (int j = 0; j < V; ++j) s[u] += TAIL && j < at.dup[k] ? 0.f : (float)xv[u][k].e[j];
         }
-        wdg_ln_row_sums<L, NT, U>(s, red);
+        wdg_ln_row_sums<L, U>(s, red);
         float d2[2 * U];                                 // sums of (x - mean) and of its square
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -150,20 +159,20 @@ __global__ void __launch_bounds__(NT) wdg_layernorm_fwd_kernel(const T* x, int64
                     d2[2 * u + 1] += d * d;
                 }
         }
-        wdg_ln_row_sums<L, NT, 2 * U>(d2, red + (L > 64 ? U * (NT / 64) : 0));
+        wdg_ln_row_sums<L, 2 * U>(d2, red + (L ? 0 : U * 16));
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int64_t p = p0 + u * RG + g;
             const float corr = d2[2 * u] * invC;
             float var = d2[2 * u + 1] * invC - corr * corr;
             var = var < 0.f ? 0.f : var;                 // (a NaN stays one)
-            const float rstd = 1.f / sqrtf(var + eps);
+            const float rstd = 1.f / sqrtf(var + eps), shift = -corr * rstd;
             if (p < P) {
 #pragma unroll
                 for (int k = 0; k < K; ++k) {
                     WdgVec<T, V> r;
 #pragma unroll
-                    for (int j = 0; j < V; ++j) r.e[j] = (T)(((((float)xv[u][k].e[j] - s[u]) - corr) * rstd) * gm[k][j] + bt[k][j]);
+                    for (int j = 0; j < V; ++j) r.e[j] = (T)fmaf(fmaf((float)xv[u][k].e[j] - s[u], rstd, shift), gm[k][j], bt[k][j]);
                     if (!TAIL || at.dup[k] < V) wdg_vec_store<T, V>(z + p * ldz + at.col[k], r);
                 }
                 if (mean_rstd && sub == 0) {
@@ -175,40 +184,58 @@ __global__ void __launch_bounds__(NT) wdg_layernorm_fwd_kernel(const T* x, int64
     }
 }
 
-// part: NULL, or one row [dgamma | dbeta] of partial sums per workgroup
+// part: NULL, or one row [dgamma | dbeta] (each of C rounded up to 4) of partial sums per workgroup
 template <class T, int V, int K, int L, int NT, int U, bool TAIL>
 __global__ void __launch_bounds__(NT) wdg_layernorm_bwd_kernel(const T* dz, int64_t lddz, const T* x, int64_t ldx,
                                                                const float* __restrict__ mean_rstd, const void* __restrict__ gamma, int ptype,
                                                                T* dx, int64_t lddx, float* part, int64_t P, int C) {
-    constexpr int RG = NT / L, COPIES = L > 64 ? RG : NT / 64;      // holders of the same columns after the sum within a wave
-    __shared__ float red[L > 64 ? 2 * 2 * U * (NT / 64) : 1];
+    constexpr int RG = L ? NT / (L ? L : 1) : 1, COPIES = L ? NT / 64 : 1;      // waves that hold sums of the same columns
+    constexpr bool AHEAD = K * U <= 2 && NT <= 512;
+    __shared__ float red[L ? 1 : 2 * 2 * U * 16];
     __shared__ float gather[COPIES > 1 ? NT * V : 1];
-    const int t = threadIdx.x, sub = t % L, g = t / L;
-    const WdgLnCols<V, K, L> at(sub, C);
+    const int lanes = L ? L : blockDim.x, t = threadIdx.x, sub = t % lanes, g = t / lanes;
+    const WdgLnCols<V, K> at(lanes, sub, C);
     const float invC = 1.f / (float)C;
     float gm[K][V], sg[K][V], sb[K][V];
 #pragma unroll
-    for (int k = 0; k < K; ++k)
+    for (int k = 0; k < K; ++k) {
+        wdg_ln_params<T, V>(gm[k], gamma, ptype, at.col[k], 1.f);
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-            gm[k][j] = wdg_ln_param<T>(gamma, ptype, at.col[k] + j, 1.f);
-            sg[k][j] = sb[k][j] = 0.f;
-        }
+        for (int j = 0; j < V; ++j) sg[k][j] = sb[k][j] = 0.f;
+    }
     int turn = 0;
-    for (int64_t p0 = (int64_t)blockIdx.x * (RG * U); p0 < P; p0 += (int64_t)gridDim.x * (RG * U)) {
-        WdgVec<T, V> xv[U][K], gv[U][K];
-        float mean[U], rstd[U], s[2 * U];
+    const int64_t stride = (int64_t)gridDim.x * (RG * U);
+    WdgVec<T, V> x_a[U][K], g_a[U][K];                   // the next rows, on their way while these are worked on (behind the last: again the last)
+    float mean_a[U], rstd_a[U];
+    auto fetch = [&](int64_t p0) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int64_t p = std::min<int64_t>(p0 + u * RG + g, P - 1);
-            mean[u] = mean_rstd[2 * p];
-            rstd[u] = mean_rstd[2 * p + 1];
+            mean_a[u] = mean_rstd[2 * p];
+            rstd_a[u] = mean_rstd[2 * p + 1];
 #pragma unroll
             for (int k = 0; k < K; ++k) {
-                xv[u][k] = wdg_vec_load<T, V>(x + p * ldx + at.col[k]);
-                gv[u][k] = wdg_vec_load<T, V>(dz + p * lddz + at.col[k]);
+                x_a[u][k] = wdg_vec_load<T, V>(x + p * ldx + at.col[k]);
+                g_a[u][k] = wdg_vec_load<T, V>(dz + p * lddz + at.col[k]);
             }
         }
+    };
+    if constexpr (AHEAD) fetch((int64_t)blockIdx.x * (RG * U));
+    for (int64_t p0 = (int64_t)blockIdx.x * (RG * U); p0 < P; p0 += stride) {
+        WdgVec<T, V> xv[U][K], gv[U][K];
+        float mean[U], rstd[U], s[2 * U];
+        if constexpr (!AHEAD) fetch(p0);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            mean[u] = mean_a[u];
+            rstd[u] = rstd_a[u];
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                xv[u][k] = x_a[u][k];
+                gv[u][k] = g_a[u][k];
+            }
+        }
+        if constexpr (AHEAD) fetch(p0 + stride);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const bool on = p0 + u * RG + g < P;
@@ -226,7 +253,7 @@ __global__ void __launch_bounds__(NT) wdg_layernorm_bwd_kernel(const T* dz, int6
                     }
                 }
         }
-        wdg_ln_row_sums<L, NT, 2 * U>(s, red + (L > 64 ? turn * 2 * U * (NT / 64) : 0));
+        wdg_ln_row_sums<L, 2 * U>(s, red + (L ? 0 : turn * 2 * U * 16));
         turn ^= 1;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -248,7 +275,8 @@ __global__ void __launch_bounds__(NT) wdg_layernorm_bwd_kernel(const T* dz, int6
     }
     if (!part) return;
     // the workgroup's sums of each column, in a fixed order: lanes of a wave that hold the same columns, then the holders through LDS
-    float* row = part + (int64_t)blockIdx.x * 2 * C;
+    const int Cp = (C + 3) & ~3;
+    float* row = part + (int64_t)blockIdx.x * 2 * Cp;
 #pragma unroll
     for (int k = 0; k < K; ++k)
 #pragma unroll
@@ -258,27 +286,33 @@ __global__ void __launch_bounds__(NT) wdg_layernorm_bwd_kernel(const T* dz, int6
             for (int j = 0; j < V; ++j) {
                 v[j] = which ? sb[k][j] : sg[k][j];
 #pragma unroll
-                for (int o = L; o < 64; o <<= 1) v[j] += __shfl_xor(v[j], o, 64);
+                for (int o = L ? L : 64; o < 64; o <<= 1) v[j] += __shfl_xor(v[j], o, 64);
             }
             if constexpr (COPIES > 1) {
-                constexpr int STEP = L > 64 ? L : 64;
                 __syncthreads();
 #pragma unroll
                 for (int j = 0; j < V; ++j) gather[j * NT + t] = v[j];
                 __syncthreads();
-                if (t < L) {
+                if (t < lanes) {
 #pragma unroll
                     for (int j = 0; j < V; ++j) {
                         v[j] = 0.f;
 #pragma unroll
-                        for (int w = 0; w < COPIES; ++w) v[j] += gather[j * NT + w * STEP + t];
+                        for (int w = 0; w < COPIES; ++w) v[j] += gather[j * NT + w * 64 + t];
                     }
                 }
             }
-            if (t < L) {
+            if (t < lanes) {
+                if (!TAIL || at.dup[k] == 0) {
+                    WdgVec<float, V> r;
 #pragma unroll
-                for (int j = 0; j < V; ++j)
-                    if (!TAIL || j >= at.dup[k]) row[which * C + at.col[k] + j] = v[j];
+                    for (int j = 0; j < V; ++j) r.e[j] = v[j];
+                    wdg_vec_store<float, V>(row + which * Cp + at.col[k], r);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < V; ++j)
+                        if (j >= at.dup[k]) row[which * Cp + at.col[k] + j] = v[j];
+                }
             }
         }
 }
@@ -401,7 +435,7 @@ __global__ void __launch_bounds__(LNW_NT) wdg_layernorm_bwd_wide_kernel(const T*
 }
 
 // ---- parameter gradients -----------------------------------------------------------------------------------------------------------
-// Partial sums [slice][dgamma | dbeta][C]: a block owns 256 V columns of one slice of the rows.
+// Partial sums [slice][dgamma | dbeta][C, rounded up to 4]: a block owns 256 V columns of one slice of the rows.
 template <class T, int V>
 __global__ void __launch_bounds__(256) wdg_layernorm_colsum_kernel(const T* __restrict__ dz, int64_t lddz, const T* __restrict__ x,
                                                                    int64_t ldx, const float* __restrict__ mean_rstd, float* part,
@@ -423,12 +457,13 @@ __global__ void __launch_bounds__(256) wdg_layernorm_colsum_kernel(const T* __re
                 sb[j] += g;
             }
     }
-    float* row = part + (int64_t)blockIdx.y * 2 * C;
+    const int64_t Cp = (C + 3) & ~3ll;
+    float* row = part + (int64_t)blockIdx.y * 2 * Cp;
 #pragma unroll
     for (int j = 0; j < V; ++j)
         if (j < n) {
             row[c + j] = sg[j];
-            row[C + c + j] = sb[j];
+            row[Cp + c + j] = sb[j];
         }
 }
 
@@ -440,11 +475,11 @@ __global__ void __launch_bounds__(1024) wdg_layernorm_finish_kernel(const float*
     constexpr int SETS = 1024 / CB;
     __shared__ float red[1024];
     const int t = threadIdx.x;
-    const int64_t col = (int64_t)blockIdx.x * CB + t % CB;
+    const int64_t col = (int64_t)blockIdx.x * CB + t % CB, Cp = (C + 3) & ~3ll;
     float s = 0.f;
-    if (col < 2 * C) {
+    if (col < 2 * Cp) {
 #pragma unroll 8
-        for (int r = t / CB; r < rows; r += SETS) s += part[(int64_t)r * 2 * C + col];
+        for (int r = t / CB; r < rows; r += SETS) s += part[(int64_t)r * 2 * Cp + col];
     }
     red[t] = s;
     __syncthreads();
@@ -452,85 +487,96 @@ __global__ void __launch_bounds__(1024) wdg_layernorm_finish_kernel(const float*
         if (t < o * CB) red[t] += red[t + o * CB];
         __syncthreads();
     }
-    if (t < CB && col < 2 * C) {
-        float* dst = col < C ? dgamma : dbeta;
-        const int64_t c = col < C ? col : col - C;
-        if (dst) dst[c] = (accumulate ? dst[c] : 0.f) + red[t];
+    if (t < CB && col < 2 * Cp) {
+        float* dst = col < Cp ? dgamma : dbeta;
+        const int64_t c = col < Cp ? col : col - Cp;
+        if (dst && c < C) dst[c] = (accumulate ? dst[c] : 0.f) + red[t];
     }
 }
 
 // ---- host side ---------------------------------------------------------------------------------------------------------------------
-// How a [P][C] tensor of vectors of V elements is cut: lanes per row, vectors per lane, threads per workgroup, rows in flight per thread.
-// L == 0: the row does not fit (the kernels that read it once per pass take it).
+// How a [P][C] tensor is cut: elements per vector, lanes per row (0: a workgroup of NT threads), vectors per lane, rows in flight per
+// thread.  K == 0: the row does not fit (the kernels that read it once per pass take it).
 struct LnGeom {
-    int L, K, NT, U, V;
-    int blocks;                                          // of the register kernels; also the rows of the backward's partial sums
-    int slices;                                          // partial sums of the column kernel (L == 0)
+    int V, L, K, NT, U;
+    int blocks;                                          // of the register kernels; rows of the backward's table of partial sums
 };
 constexpr int LN_CUS = 256;
+constexpr int64_t LN_MAX_ROW = 16384;                    // widest row that a workgroup holds in registers
 
 static LnGeom ln_geom(int64_t P, int64_t C, int type, bool bwd) {
-    LnGeom g = {0, 1, 256, 1, type == WDG_F32 ? 4 : 8, 1, 0};
+    LnGeom g = {type == WDG_F32 ? 4 : 8, 0, 0, 256, 1, 0};
     if (C < g.V) {
         g.V = 1;
         g.L = 8;
+        g.K = 1;
         g.U = 4;
     } else {
         const int64_t vecs = (C + g.V - 1) / g.V;
-        const int most = g.V == 4 ? 4 : 2;               // vectors per lane: 16 elements, so that three fp32 values per column fit
+        const int wave = g.V == 4 ? 4 : 2;               // vectors per lane of a row that one wave holds: at most 16 elements
         if (vecs <= 64) {
             g.L = 1;
             while (g.L < vecs) g.L <<= 1;
+            g.K = 1;
             g.U = 4;
-        } else if (vecs <= 64 * most) {
+        } else if (vecs <= 64 * wave) {
             g.L = 64;
             g.K = vecs <= 128 ? 2 : 4;
             g.U = 4 / g.K;
-        } else if (vecs <= 1024 * most) {
-            g.L = vecs <= 256 * most ? 256 : vecs <= 512 * most ? 512 : 1024;
-            g.K = vecs <= 256 * (most / 2) ? most / 2 : most;
-            g.NT = g.L;
-            g.U = 1;
+        } else if (C <= LN_MAX_ROW) {
+            g.K = wave;
+            g.NT = (int)((vecs + 64 * g.K - 1) / (64 * g.K)) * 64;
+            // Forward, 16-bit types: two rows per barrier, except in workgroups of 5 to 8 waves (us with one / two rows: 16384 x 4096
+            // 54.4 / 50.5, 16384 x 10000 157 / 131, but 16384 x 8192 97 / 104 and 16384 x 5003 68 / 74).  With 32-bit elements twice
+            // the bytes per row are on their way already: 16384 x 4096 97 / 101, 4096 x 16384 97 / 115.
+            g.U = !bwd && g.V == 8 && (g.NT <= 256 || g.NT > 512) ? 2 : 1;
         }
     }
-    if (g.L) {
-        const int64_t rows = (int64_t)(g.NT / g.L) * g.U, resident = (int64_t)LN_CUS * (bwd ? 1024 : 2048) / g.NT;
+    if (g.K) {
+        // Threads per compute unit: a workgroup that stays walks over many rows with its parameters in registers, and each one of the
+        // backward writes 8 C bytes of partial sums, so no more of them than keep the memory busy.  Backward, us with 512 / 1024:
+        // 16384 x 4096 bf16 81 / 94, 32768 x 2048 bf16 81 / 95, 262144 x 256 fp32 151 / 156.  Forward, us with 1024 / 2048: 16384 x 4097
+        // bf16 (320 threads) 65 / 78, 16384 x 5003 fp16 68 / 75; 4194304 x 16 bf16 57 / 57, 32768 x 2048 bf16 51 / 51.
+        const int threads = bwd ? 512 : g.NT > 256 ? 1024 : 2048;
+        const int64_t rows = (int64_t)(g.L ? g.NT / g.L : 1) * g.U, resident = LN_CUS * std::max(1, threads / g.NT);
         g.blocks = (int)std::max<int64_t>(1, std::min<int64_t>((P + rows - 1) / rows, resident));
     } else {
         const int64_t tiles = (C + 256 * g.V - 1) / (256 * g.V);
-        g.slices = (int)std::max<int64_t>(1, std::min<int64_t>((P + 15) / 16, std::max<int64_t>(1, 1024 / tiles)));
+        g.blocks = (int)std::max<int64_t>(1, std::min<int64_t>((P + 15) / 16, std::max<int64_t>(1, 1024 / tiles)));
     }
     return g;
 }
 
-// F::template run<V, K, L, NT, U>() for the geometry; false: no register kernel for it
+// f.template run<V, K, L, NT, U>() for the geometry, NT the most threads the instance is built for; false: no register kernel for it
+template <int V, int U, class F>
+static void ln_dispatch_block(const LnGeom& g, F& f) {
+    constexpr int K = V == 4 ? 4 : 2;
+    if (g.NT <= 256) f.template run<V, K, 0, 256, U>();
+    else if (g.NT <= 512) f.template run<V, K, 0, 512, 1>();
+    else f.template run<V, K, 0, 1024, U>();
+}
 template <int V, class F>
-static bool ln_dispatch(const LnGeom& g, F&& f) {
-    if (V == 1) {
+static bool ln_dispatch(const LnGeom& g, F& f) {
+    if (g.K == 0) return false;
+    if (g.V == 1) {
         f.template run<1, 1, 8, 256, 4>();
         return true;
     }
-    constexpr int M = V == 4 ? 4 : 2;
     switch (g.L) {
-        case 1: f.template run<V, 1, 1, 256, 4>(); return true;
-        case 2: f.template run<V, 1, 2, 256, 4>(); return true;
-        case 4: f.template run<V, 1, 4, 256, 4>(); return true;
-        case 8: f.template run<V, 1, 8, 256, 4>(); return true;
-        case 16: f.template run<V, 1, 16, 256, 4>(); return true;
-        case 32: f.template run<V, 1, 32, 256, 4>(); return true;
+        case 1: f.template run<V, 1, 1, 256, 4>(); break;
+        case 2: f.template run<V, 1, 2, 256, 4>(); break;
+        case 4: f.template run<V, 1, 4, 256, 4>(); break;
+        case 8: f.template run<V, 1, 8, 256, 4>(); break;
+        case 16: f.template run<V, 1, 16, 256, 4>(); break;
+        case 32: f.template run<V, 1, 32, 256, 4>(); break;
         case 64:
             if (g.K == 1) f.template run<V, 1, 64, 256, 4>();
             else if (g.K == 2) f.template run<V, 2, 64, 256, 2>();
-            else f.template run<V, M, 64, 256, 1>();
-            return true;
-        case 256:
-            if (g.K == M) f.template run<V, M, 256, 256, 1>();
-            else f.template run<V, M / 2, 256, 256, 1>();
-            return true;
-        case 512: f.template run<V, M, 512, 512, 1>(); return true;
-        case 1024: f.template run<V, M, 1024, 1024, 1>(); return true;
+            else if constexpr (V == 4) f.template run<V, 4, 64, 256, 1>();
+            break;
+        default: ln_dispatch_block<V, V == 8 ? F::BLOCK_U16 : 1>(g, f);
     }
-    return false;
+    return true;
 }
 
 static bool ln_types_ok(int type, int ptype) {
@@ -540,6 +586,7 @@ static const int64_t LN_MAX_C = 1ll << 24;      // (c / C and the sums' fp32 sca
 
 template <class T>
 struct LnFwd {
+    static constexpr int BLOCK_U16 = 2;
     const T* x;
     int64_t ldx;
     const void *gamma, *beta;
@@ -553,10 +600,10 @@ struct LnFwd {
     LnGeom g;
     template <int V, int K, int L, int NT, int U>
     void run() {
-        if (C == (int64_t)V * K * L)
-            hipLaunchKernelGGL((wdg_layernorm_fwd_kernel<T, V, K, L, NT, U, false>), dim3(g.blocks), dim3(NT), 0, st, x, ldx, gamma, beta, ptype, eps, z, ldz, mean_rstd, P, (int)C);
+        if (C == (int64_t)V * K * (L ? L : g.NT))
+            hipLaunchKernelGGL((wdg_layernorm_fwd_kernel<T, V, K, L, NT, U, false>), dim3(g.blocks), dim3(g.NT), 0, st, x, ldx, gamma, beta, ptype, eps, z, ldz, mean_rstd, P, (int)C);
         else
-            hipLaunchKernelGGL((wdg_layernorm_fwd_kernel<T, V, K, L, NT, U, true>), dim3(g.blocks), dim3(NT), 0, st, x, ldx, gamma, beta, ptype, eps, z, ldz, mean_rstd, P, (int)C);
+            hipLaunchKernelGGL((wdg_layernorm_fwd_kernel<T, V, K, L, NT, U, true>), dim3(g.blocks), dim3(g.NT), 0, st, x, ldx, gamma, beta, ptype, eps, z, ldz, mean_rstd, P, (int)C);
     }
 };
 
@@ -564,8 +611,7 @@ template <class T, int V>
 static int ln_fwd_launch(const void* x, int64_t ldx, const void* gamma, const void* beta, int ptype, float eps, void* z, int64_t ldz,
                          float* mean_rstd, int64_t P, int64_t C, int type, hipStream_t st) {
     LnFwd<T> f = {(const T*)x, ldx, gamma, beta, ptype, eps, (T*)z, ldz, mean_rstd, P, C, st, ln_geom(P, C, type, false)};
-    if (f.g.V == 1) ln_dispatch<1>(f.g, f);
-    else if (!ln_dispatch<V>(f.g, f))
+    if (!ln_dispatch<V>(f.g, f))
         hipLaunchKernelGGL((wdg_layernorm_fwd_wide_kernel<T, V>), dim3((unsigned)std::min<int64_t>(P, 4096)), dim3(LNW_NT), 0, st, (const T*)x, ldx,
                            gamma, beta, ptype, eps, (T*)z, ldz, mean_rstd, P, C);
     WDG_LAUNCH_CHECK();
@@ -588,20 +634,22 @@ extern "C" int wdg_layernorm_fwd(const void* x, int64_t ldx, const void* gamma, 
 extern "C" size_t wdg_layernorm_bwd_ws_bytes(int64_t P, int64_t C, int type) {
     if (P <= 0 || C <= 0 || C > LN_MAX_C || type < WDG_F32 || type > WDG_F16) return 0;
     const LnGeom g = ln_geom(P, C, type, true);
-    return (size_t)(g.L ? g.blocks : g.slices) * 2 * (size_t)C * sizeof(float);
+    return (size_t)g.blocks * 2 * (size_t)((C + 3) & ~3ll) * sizeof(float);
 }
 
 static int ln_finish(const float* part, int rows, int64_t C, float* dgamma, float* dbeta, int accumulate, hipStream_t st) {
-    if (2 * C <= 256)
-        hipLaunchKernelGGL(wdg_layernorm_finish_kernel<16>, dim3((unsigned)((2 * C + 15) / 16)), dim3(1024), 0, st, part, rows, C, dgamma, dbeta, accumulate);
+    const int64_t cols = 2 * ((C + 3) & ~3ll);
+    if (cols <= 256)
+        hipLaunchKernelGGL(wdg_layernorm_finish_kernel<16>, dim3((unsigned)((cols + 15) / 16)), dim3(1024), 0, st, part, rows, C, dgamma, dbeta, accumulate);
     else
-        hipLaunchKernelGGL(wdg_layernorm_finish_kernel<64>, dim3((unsigned)((2 * C + 63) / 64)), dim3(1024), 0, st, part, rows, C, dgamma, dbeta, accumulate);
+        hipLaunchKernelGGL(wdg_layernorm_finish_kernel<64>, dim3((unsigned)((cols + 63) / 64)), dim3(1024), 0, st, part, rows, C, dgamma, dbeta, accumulate);
     WDG_LAUNCH_CHECK();
     return WDG_OK;
 }
 
 template <class T>
 struct LnBwd {
+    static constexpr int BLOCK_U16 = 1;
     const T* dz;
     int64_t lddz;
     const T* x;
@@ -617,10 +665,10 @@ struct LnBwd {
     LnGeom g;
     template <int V, int K, int L, int NT, int U>
     void run() {
-        if (C == (int64_t)V * K * L)
-            hipLaunchKernelGGL((wdg_layernorm_bwd_kernel<T, V, K, L, NT, U, false>), dim3(g.blocks), dim3(NT), 0, st, dz, lddz, x, ldx, mean_rstd, gamma, ptype, dx, lddx, part, P, (int)C);
+        if (C == (int64_t)V * K * (L ? L : g.NT))
+            hipLaunchKernelGGL((wdg_layernorm_bwd_kernel<T, V, K, L, NT, U, false>), dim3(g.blocks), dim3(g.NT), 0, st, dz, lddz, x, ldx, mean_rstd, gamma, ptype, dx, lddx, part, P, (int)C);
         else
-            hipLaunchKernelGGL((wdg_layernorm_bwd_kernel<T, V, K, L, NT, U, true>), dim3(g.blocks), dim3(NT), 0, st, dz, lddz, x, ldx, mean_rstd, gamma, ptype, dx, lddx, part, P, (int)C);
+            hipLaunchKernelGGL((wdg_layernorm_bwd_kernel<T, V, K, L, NT, U, true>), dim3(g.blocks), dim3(g.NT), 0, st, dz, lddz, x, ldx, mean_rstd, gamma, ptype, dx, lddx, part, P, (int)C);
     }
 };
 
@@ -631,20 +679,17 @@ static int ln_bwd_launch(const void* dz, int64_t lddz, const void* x, int64_t ld
     const bool params = dgamma || dbeta;
     if (P == 0) return params ? ln_finish(part, 0, C, dgamma, dbeta, accumulate, st) : WDG_OK;
     LnBwd<T> f = {(const T*)dz, lddz, (const T*)x, ldx, mean_rstd, gamma, ptype, (T*)dx, lddx, params ? part : nullptr, P, C, st, ln_geom(P, C, type, true)};
-    int rows = f.g.blocks;
-    if (f.g.V == 1) ln_dispatch<1>(f.g, f);
-    else if (!ln_dispatch<V>(f.g, f)) {
+    if (!ln_dispatch<V>(f.g, f)) {
         if (params) {
-            rows = f.g.slices;
-            hipLaunchKernelGGL((wdg_layernorm_colsum_kernel<T, V>), dim3((unsigned)((C + 256 * V - 1) / (256 * V)), rows), dim3(256), 0, st,
-                               (const T*)dz, lddz, (const T*)x, ldx, mean_rstd, part, P, C, rows);
+            hipLaunchKernelGGL((wdg_layernorm_colsum_kernel<T, V>), dim3((unsigned)((C + 256 * V - 1) / (256 * V)), f.g.blocks), dim3(256), 0, st,
+                               (const T*)dz, lddz, (const T*)x, ldx, mean_rstd, part, P, C, f.g.blocks);
             WDG_LAUNCH_CHECK();
         }
         hipLaunchKernelGGL((wdg_layernorm_bwd_wide_kernel<T, V>), dim3((unsigned)std::min<int64_t>(P, 4096)), dim3(LNW_NT), 0, st, (const T*)dz,
                            lddz, (const T*)x, ldx, mean_rstd, gamma, ptype, (T*)dx, lddx, P, C);
     }
     WDG_LAUNCH_CHECK();
-    return params ? ln_finish(part, rows, C, dgamma, dbeta, accumulate, st) : WDG_OK;
+    return params ? ln_finish(part, f.g.blocks, C, dgamma, dbeta, accumulate, st) : WDG_OK;
 }
 
 extern "C" int wdg_layernorm_bwd(const void* dz, int64_t lddz, const void* x, int64_t ldx, const float* mean_rstd, const void* gamma,
