@@ -41,8 +41,12 @@ def test_forward_refuses_overlap(ops):
     h = torch.zeros(6, 10, dtype=torch.bfloat16)
     with pytest.raises(ValueError, match="one type"):
         ops.layernorm_fwd(**{**args(), "x": h, "z": torch.zeros_like(h), "gamma": torch.ones(10, dtype=torch.bfloat16)})
-    assert not ops._overlap(buf[:, :10], buf[:, 10:20]) and not ops._overlap(buf[:, 14:24], buf[:, :10])      # two halves of a concatenation
-    assert not ops._overlap(buf[:3], buf[3:]) and ops._overlap(buf[:, :10], buf[:, 9:19])
+    rows = lambda t: ops._ln_rows("x", t, t)      # noqa: E731
+    for a, b in ((buf[:, :10], buf[:, 10:20]), (buf[:, 14:24], buf[:, :10]), (buf[:, :10], buf[:, 14:]), (buf[:3], buf[3:]), (buf, buf)):      # two halves of a concatenation
+        ops._ln_apart("z", rows(a), {"x": rows(b)}, a.shape[1], 4)
+    for a, b in ((buf[:, :10], buf[:, 9:19]), (buf[:, 9:19], buf[:, :10]), (buf[:3, 1:], buf[2:5, 1:])):
+        with pytest.raises(ValueError, match="overlaps"):
+            ops._ln_apart("z", rows(a), {"x": rows(b)}, a.shape[1], 4)
 
 
 @pytest.mark.parametrize("change", [

@@ -219,7 +219,7 @@ class _AdamWBatch:
         ops._on_device(*state)
         if len(state) != len(kinds) or any(t.dtype != d or tuple(t.shape) != (n,) or not t.is_contiguous() for t, (d, n) in zip(state, kinds)):
             raise ValueError("state: flat contiguous tensors " + ", ".join(f"{d} [{n}]" for d, n in kinds) + " are wanted")
-        self.state = state
+        self.state = tuple(state)
         self.m, self.v = state[:2]
         self.m_scale, self.v_scale = state[2:] if state_bits == 8 else (None, None)
         self.handle = None
@@ -235,18 +235,20 @@ class _AdamWBatch:
         self.scratch_bytes = int(ops.lib.wdg_adamw_scratch_bytes())
         need = int(ops.lib.wdg_adamw_table_bytes(handle))
         self.table = torch.empty(max(need, 16), dtype=torch.uint8, device=ops.device)
-        self.home = ops.stream
-        with torch.cuda.device(ops.device):
-            native.check(ops.lib.wdg_adamw_bind(handle, self.table.data_ptr(), need, self.home), "adamw_bind")
+        self.home = ops._raw_stream()
+        native.check(ops.lib.wdg_adamw_bind(handle, self.table.data_ptr(), need, self.home), "adamw_bind")
 
-    def _launch(self):
-        """(scratch, stream) of one call: the scratch is the call's own (the allocator orders its reuse on this stream, and inside a
-        graph capture it belongs to the graph); what the batch owns is kept from reuse while another stream than its own works on it."""
-        stream = self.ops.stream
+    def _launch_stream(self):
+        """The stream of one call; what the batch owns is kept from reuse while another stream than its own works on it."""
+        stream = self.ops._raw_stream()
         if stream != self.home and not torch.cuda.is_current_stream_capturing():
             for t in (self.table, *self.state):
                 t.record_stream(torch.cuda.current_stream(self.ops.device))
-        return torch.empty(self.scratch_bytes // 8, dtype=torch.float64, device=self.ops.device), stream
+        return stream
+
+    def _scratch(self):
+        """Scratch of one call alone: the allocator orders its reuse on this stream, and inside a graph capture it belongs to the graph."""
+        return torch.empty(self.scratch_bytes // 8, dtype=torch.float64, device=self.ops.device)
 
     def _norm_ptr(self, norm):
         if norm is not None:
@@ -271,18 +273,17 @@ class _AdamWBatch:
             args.step_dev = t.data_ptr()
         else:
             args.step = t
-        with torch.cuda.device(self.ops.device):
-            scratch, stream = self._launch()
-            native.check(self.ops.lib.wdg_adamw_step(self.handle, C.byref(args), scratch.data_ptr(), self.scratch_bytes, stream), "adamw_step")
+        stream = self._launch_stream()
+        scratch = self._scratch() if max_norm is not None else None
+        native.check(self.ops.lib.wdg_adamw_step(self.handle, C.byref(args), _ptr(scratch), self.scratch_bytes, stream), "adamw_step")
 
     def grad_norm(self, norm, grad_scale=1.0):
         """norm[0] = grad_scale * sqrt(sum of all gradients' squares), on the device."""
         if norm is None:
             raise ValueError("norm: one fp32 value is wanted")
         p = self._norm_ptr(norm)
-        with torch.cuda.device(self.ops.device):
-            scratch, stream = self._launch()
-            native.check(self.ops.lib.wdg_adamw_grad_norm(self.handle, grad_scale, p, scratch.data_ptr(), self.scratch_bytes, stream), "adamw_grad_norm")
+        stream, scratch = self._launch_stream(), self._scratch()
+        native.check(self.ops.lib.wdg_adamw_grad_norm(self.handle, grad_scale, p, scratch.data_ptr(), self.scratch_bytes, stream), "adamw_grad_norm")
 
     def moments(self, m_out=None, v_out=None):
         """The moments as numbers, in the state's flat layout: into m_out / v_out ([total], one type of fp32, bf16, fp16)."""
@@ -297,10 +298,9 @@ class _AdamWBatch:
             return
         if not outs:
             return
-        with torch.cuda.device(self.ops.device):
-            native.check(self.ops.lib.wdg_adamw_moments(self.m.data_ptr(), self.m_scale.data_ptr(), self.v.data_ptr(), self.v_scale.data_ptr(),
-                                                        self.total // self.BLOCK, _ptr(m_out), _ptr(v_out), self.ops.TYPES[outs[0].dtype],
-                                                        self.ops.stream), "adamw_moments")
+        native.check(self.ops.lib.wdg_adamw_moments(self.m.data_ptr(), self.m_scale.data_ptr(), self.v.data_ptr(), self.v_scale.data_ptr(),
+                                                    self.total // self.BLOCK, _ptr(m_out), _ptr(v_out), self.ops.TYPES[outs[0].dtype],
+                                                    self._launch_stream()), "adamw_moments")
 
     def __del__(self):
         try:
@@ -348,6 +348,8 @@ class HipOps:
                                      "there is no CPU execution path in this package")
         self.device = torch.device(device if device is not None else f"cuda:{torch.cuda.current_device()}")
         torch.cuda.set_device(self.device)
+        if self.device.index is None:                     # ("cuda": the current one)
+            self.device = torch.device("cuda", torch.cuda.current_device())
         self.lib = native.load()
         self._plans = {}
         self._ws = None
@@ -1134,99 +1136,99 @@ class HipOps:
             if t is not None and t.device != self.device:
                 raise ValueError(f"tensor on {t.device}, this backend runs on {self.device}")
 
-    @staticmethod
-    def _overlap(a, b):
-        """Whether two tensors may share memory: the address ranges they span meet, and they are not two sets of columns of one buffer."""
-        if a is None or b is None or not a.numel() or not b.numel():
-            return False
-        pa, pb, es = a.data_ptr(), b.data_ptr(), a.element_size()
-        end = lambda t, p: p + t.element_size() * (1 + sum((n - 1) * abs(st) for n, st in zip(t.shape, t.stride())))      # noqa: E731
-        if pa >= end(b, pb) or pb >= end(a, pa):
-            return False
-        if a.dim() == b.dim() == 2 and es == b.element_size() and a.stride() == b.stride() and a.stride(1) == 1 and (pb - pa) % es == 0:
-            ld = a.stride(0)
-            off = ((pb - pa) // es) % ld if ld > 0 else 0
-            return not (off >= a.shape[1] and off + b.shape[1] <= ld)
-        return True
+    def _raw_stream(self):
+        """The current stream of this backend's device as the C ABI takes it, and that device made current: a call costs about as much host
+        time as its launch, and the stream object of the `stream` property alone is a quarter of that."""
+        index = self.device.index
+        if torch.cuda.current_device() != index:
+            torch.cuda.set_device(index)
+        return torch._C._cuda_getCurrentRawStream(index)
 
-    def _ln_rows(self, name, t, like=None, out=False):
-        """(ptr, row stride) of a [P, C] tensor of layernorm_fwd / _bwd; `out`: rows are written, so they may not overlap."""
-        if t.dim() != 2 or t.dtype not in self.TYPES:
-            raise ValueError(f"{name}: a [P, C] tensor of {', '.join(str(d) for d in self.TYPES)} is wanted, got {t.dtype} {tuple(t.shape)}")
-        if like is not None and (t.shape != like.shape or t.dtype != like.dtype):
-            raise ValueError(f"{name}: {t.dtype} {tuple(t.shape)}, but {like.dtype} {tuple(like.shape)} goes with it")
-        P, Cn = t.shape
-        if Cn < 1 or (Cn > 1 and t.stride(1) != 1) or (out and P > 1 and t.stride(0) < Cn):
-            raise ValueError(f"{name}: shape {tuple(t.shape)}, strides {t.stride()}: channels have to be adjacent" + (" and rows apart" if out else ""))
-        return t.data_ptr(), t.stride(0) if P > 1 else Cn
+    def _ln_rows(self, name, t, like, out=False):
+        """(address, row stride, end of the last row) of a [P, C] tensor of layernorm_fwd / _bwd; `out`: rows are written, so they may not overlap."""
+        shape, st = t.shape, t.stride()
+        if len(shape) != 2 or t.dtype not in self.TYPES or t.dtype is not like.dtype or shape != like.shape:
+            raise ValueError(f"{name}: a [P, C] tensor of {', '.join(str(d) for d in self.TYPES)} is wanted, of one shape and type with the others: "
+                             f"{t.dtype} {tuple(shape)}, {like.dtype} {tuple(like.shape)}")
+        if t.device != self.device:
+            raise ValueError(f"{name} is on {t.device}, this backend runs on {self.device}")
+        P, Cn = shape
+        ld = st[0] if P > 1 else Cn
+        if Cn < 1 or (Cn > 1 and st[1] != 1) or (out and ld < Cn):
+            raise ValueError(f"{name}: shape {tuple(shape)}, strides {st}: channels have to be adjacent" + (" and rows apart" if out else ""))
+        p = t.data_ptr()
+        return p, ld, p + ((P - 1) * ld + Cn) * t.element_size() if P else p
 
     def _ln_vec(self, name, v, Cn, dtypes):
-        if v is not None and (v.dtype not in dtypes or tuple(v.shape) != (Cn,) or not v.is_contiguous()):
-            raise ValueError(f"{name}: a contiguous [{Cn}] vector of {' or '.join(str(d) for d in dtypes)} is wanted, got {v.dtype} {tuple(v.shape)}")
-        return v
-
-    def _ln_params(self, x, gamma, beta=None):
-        """wdg_type of the parameters: fp32 or the activations' (both the same)."""
-        for name, v in (("gamma", gamma), ("beta", beta)):
-            self._ln_vec(name, v, x.shape[1], (torch.float32, x.dtype))
-        kinds = {v.dtype for v in (gamma, beta) if v is not None}
-        if len(kinds) > 1:
-            raise ValueError("gamma and beta have to be of one type")
-        return self.TYPES[kinds.pop()] if kinds else 0
+        """(address, end) of a [C] vector, (0, 0) for None."""
+        if v is None:
+            return 0, 0
+        if v.dtype not in dtypes or v.dim() != 1 or v.shape[0] != Cn or not v.is_contiguous() or v.device != self.device:
+            raise ValueError(f"{name}: a contiguous [{Cn}] vector of {' or '.join(str(d) for d in dtypes)} on {self.device} is wanted, got {v.dtype} {tuple(v.shape)} on {v.device}")
+        p = v.data_ptr()
+        return p, p + Cn * v.element_size()
 
     def _ln_stats(self, mean_rstd, P):
-        if mean_rstd is not None and (mean_rstd.dtype != torch.float32 or tuple(mean_rstd.shape) != (P, 2) or not mean_rstd.is_contiguous()):
-            raise ValueError(f"mean_rstd: a contiguous fp32 [{P}, 2] tensor is wanted, got {mean_rstd.dtype} {tuple(mean_rstd.shape)}")
-        return _ptr(mean_rstd)
+        if mean_rstd is None:
+            return 0, 0
+        if mean_rstd.dtype is not torch.float32 or mean_rstd.shape != (P, 2) or not mean_rstd.is_contiguous() or mean_rstd.device != self.device:
+            raise ValueError(f"mean_rstd: a contiguous fp32 [{P}, 2] tensor on {self.device} is wanted, got {mean_rstd.dtype} {tuple(mean_rstd.shape)} on {mean_rstd.device}")
+        p = mean_rstd.data_ptr()
+        return p, p + 8 * P
 
-    def _ln_apart(self, out_name, out, **others):
-        """`out` is written: it may be one of `others` element for element, and meets none of them otherwise."""
-        for name, t in others.items():
-            same = t is not None and t.data_ptr() == out.data_ptr() and t.shape == out.shape and t.stride() == out.stride() and t.dtype == out.dtype
-            if not same and self._overlap(out, t):
+    @staticmethod
+    def _ln_apart(out_name, out, others, Cn, size):
+        """The written range `out` = (address, end) or rows (address, stride, end) meets none of `others` ({name: the same}).  Rows may be
+        another tensor's element for element, or other columns of one buffer."""
+        for name, o in others.items():
+            if out[0] < o[-1] and o[0] < out[-1]:
+                if len(o) == len(out) == 3 and o[1] == out[1]:
+                    off = (o[0] - out[0]) % (out[1] * size)
+                    if o[0] == out[0] or (Cn * size <= off <= (out[1] - Cn) * size):
+                        continue
                 raise ValueError(f"{out_name} overlaps {name}")
 
     def layernorm_fwd(self, x, gamma, beta, eps, z, mean_rstd=None):
         """z = (x - mean) / sqrt(var + eps) * gamma + beta over the last axis of x [P, C], C >= 1 any width, x and z fp32, bf16 or
         fp16 with adjacent channels and any row stride (wdg_layernorm_fwd).  gamma, beta: [C], fp32 or x's type, or None; mean_rstd:
         fp32 [P, 2], kept for layernorm_bwd, or None.  z may be x."""
-        self._on_device(x, gamma, beta, z, mean_rstd)
-        px, ldx = self._ln_rows("x", x)
-        pz, ldz = self._ln_rows("z", z, like=x, out=True)
-        kind = self._ln_params(x, gamma, beta)
-        stats = self._ln_stats(mean_rstd, x.shape[0])
-        self._ln_apart("z", z, x=x, gamma=gamma, beta=beta)
-        if mean_rstd is not None:
-            self._ln_apart("mean_rstd", mean_rstd, x=x, z=z, gamma=gamma, beta=beta)
-        with torch.cuda.device(self.device):
-            native.check(self.lib.wdg_layernorm_fwd(px, ldx, _ptr(gamma), _ptr(beta), float(eps), pz, ldz, stats, x.shape[0], x.shape[1],
-                                                    self.TYPES[x.dtype], kind, self.stream), "layernorm_fwd")
+        xr, zr = self._ln_rows("x", x, x), self._ln_rows("z", z, x, out=True)
+        P, Cn = x.shape
+        kinds = (torch.float32, x.dtype)
+        ga, be, mr = self._ln_vec("gamma", gamma, Cn, kinds), self._ln_vec("beta", beta, Cn, kinds), self._ln_stats(mean_rstd, P)
+        if gamma is not None and beta is not None and gamma.dtype is not beta.dtype:
+            raise ValueError("gamma and beta have to be of one type")
+        par = gamma if gamma is not None else beta
+        size = x.element_size()
+        self._ln_apart("z", zr, {"x": xr, "gamma": ga, "beta": be, "mean_rstd": mr}, Cn, size)
+        if mr[0]:
+            self._ln_apart("mean_rstd", mr, {"x": xr, "gamma": ga, "beta": be}, Cn, size)
+        native.check(self.lib.wdg_layernorm_fwd(xr[0], xr[1], ga[0], be[0], eps, zr[0], zr[1], mr[0], P, Cn, self.TYPES[x.dtype],
+                                                self.TYPES[par.dtype] if par is not None else 0, self._raw_stream()), "layernorm_fwd")
 
     def layernorm_bwd(self, dz, x, mean_rstd, gamma, dx, dgamma=None, dbeta=None, accumulate=True):
         """Gradients of layernorm_fwd: dx (may be dz or x), and dgamma / dbeta (fp32 [C], added to unless accumulate is False;
         None: not formed), summed over the rows in a fixed order (wdg_layernorm_bwd)."""
-        self._on_device(dz, x, mean_rstd, gamma, dx, dgamma, dbeta)
-        px, ldx = self._ln_rows("x", x)
-        pg, ldg = self._ln_rows("dz", dz, like=x)
-        pd, ldd = self._ln_rows("dx", dx, like=x, out=True)
+        xr, gr, dr = self._ln_rows("x", x, x), self._ln_rows("dz", dz, x), self._ln_rows("dx", dx, x, out=True)
         P, Cn = x.shape
-        kind = self._ln_params(x, gamma)
         if mean_rstd is None:
             raise ValueError("mean_rstd of the forward pass is needed")
-        stats = self._ln_stats(mean_rstd, P)
-        self._ln_apart("dx", dx, x=x, dz=dz, mean_rstd=mean_rstd, gamma=gamma)
-        for name, v in (("dgamma", dgamma), ("dbeta", dbeta)):
-            if self._ln_vec(name, v, Cn, (torch.float32,)) is not None:
-                if any(self._overlap(v, o) for o in (x, dz, dx, mean_rstd, gamma)):
-                    raise ValueError(f"{name} overlaps another argument")
-        if self._overlap(dgamma, dbeta):
-            raise ValueError("dgamma overlaps dbeta")
-        with torch.cuda.device(self.device):
+        ga, mr = self._ln_vec("gamma", gamma, Cn, (torch.float32, x.dtype)), self._ln_stats(mean_rstd, P)
+        dg, db = self._ln_vec("dgamma", dgamma, Cn, (torch.float32,)), self._ln_vec("dbeta", dbeta, Cn, (torch.float32,))
+        read = {"x": xr, "dz": gr, "mean_rstd": mr, "gamma": ga}
+        size, kind = x.element_size(), self.TYPES[x.dtype]
+        self._ln_apart("dx", dr, read, Cn, size)
+        need, ws, wp = 0, None, 0
+        if dg[0] or db[0]:
+            read["dx"] = dr
+            self._ln_apart("dgamma", dg, read, Cn, size)
+            self._ln_apart("dbeta", db, {**read, "dgamma": dg}, Cn, size)
             # scratch of this call alone: the allocator orders its reuse on this stream, and inside a graph capture it belongs to the graph
-            need = int(self.lib.wdg_layernorm_bwd_ws_bytes(P, Cn, self.TYPES[x.dtype])) if dgamma is not None or dbeta is not None else 0
-            ws = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
-            native.check(self.lib.wdg_layernorm_bwd(pg, ldg, px, ldx, stats, _ptr(gamma), pd, ldd, _ptr(dgamma), _ptr(dbeta), int(bool(accumulate)),
-                                                    P, Cn, self.TYPES[x.dtype], kind, _ptr(ws), need, self.stream), "layernorm_bwd")
+            need = self.lib.wdg_layernorm_bwd_ws_bytes(P, Cn, kind)
+            ws = torch.empty(need, dtype=torch.uint8, device=self.device)
+            wp = ws.data_ptr()
+        native.check(self.lib.wdg_layernorm_bwd(gr[0], gr[1], xr[0], xr[1], mr[0], ga[0], dr[0], dr[1], dg[0], db[0], bool(accumulate), P, Cn,
+                                                kind, self.TYPES[gamma.dtype] if gamma is not None else 0, wp, need, self._raw_stream()), "layernorm_bwd")
 
     # ---- ConvLSTM cell ----------------------------------------------------------------------
     def lstm_fwd(self, gates, c_prev, c, h, F):
