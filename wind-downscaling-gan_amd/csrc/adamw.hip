@@ -11,9 +11,10 @@
 #include <math.h>
 #include <vector>
 
-constexpr int AW_CHUNK = 4096;     // elements per record
+constexpr int AW_CHUNK = 4096;     // elements per record; AW_SMALL of them in short lists (aw_chunk_size)
+constexpr int AW_SMALL = 1024;
 constexpr int AW_BLOCK = 256;      // elements that share a scale of the 8-bit states
-constexpr int AW_PARTS = 512;      // partial sums of the gradient norm
+constexpr int AW_PARTS = 256;      // partial sums of the gradient norm: one for each thread of the step's workgroups
 
 struct WdgAdamwChunk {
     void* p;
@@ -23,7 +24,7 @@ struct WdgAdamwChunk {
     float* ms;
     float* vs;
     void* copy;
-    int n;                                        // elements, 1 .. AW_CHUNK
+    int n;                                        // elements, 1 .. the batch's chunk size
     unsigned char p_type, g_type, copy_type, pad; // copy_type 0: no copy
     float decay;
     int pad2;
@@ -31,6 +32,8 @@ struct WdgAdamwChunk {
 struct wdg_adamw_batch {
     std::vector<WdgAdamwChunk> chunks;
     int bits = 32;
+    int chunk = AW_CHUNK;
+    int64_t bytes = 0, grad_bytes = 0;            // of everything a step touches, of the gradients alone
     const WdgAdamwChunk* table = nullptr;         // device memory of the caller
 };
 
@@ -48,31 +51,31 @@ struct WdgAdamwHyper {
 };
 
 // ---- four elements of a tensor, the missing ones of its last quad read as zero ----------------------------------------------------
-template <class T>
+template <bool STREAM = false, class T>
 __device__ __forceinline__ f32x4 wdg_aw_load(const T* p, int n) {
     f32x4 r = {0.f, 0.f, 0.f, 0.f};
     if (n >= 4) {
-        const WdgVec<T, 4> v = wdg_vec_load<T, 4>(p);
+        const WdgVec<T, 4> v = wdg_vec_load<T, 4, STREAM>(p);
 #pragma unroll
         for (int j = 0; j < 4; ++j) r[j] = (float)v.e[j];
     } else {
 #pragma unroll
         for (int j = 0; j < 3; ++j)
-            if (j < n) r[j] = (float)p[j];
+            if (j < n) r[j] = (float)((const WDG_GLOBAL T*)p)[j];
     }
     return r;
 }
-template <class T>
+template <bool STREAM = false, class T>
 __device__ __forceinline__ void wdg_aw_store(T* p, int n, const f32x4& r) {
     if (n >= 4) {
         WdgVec<T, 4> v;
 #pragma unroll
         for (int j = 0; j < 4; ++j) v.e[j] = (T)r[j];
-        wdg_vec_store<T, 4>(p, v);
+        wdg_vec_store<T, 4, STREAM>(p, v);
     } else {
 #pragma unroll
         for (int j = 0; j < 3; ++j)
-            if (j < n) p[j] = (T)r[j];
+            if (j < n) ((WDG_GLOBAL T*)p)[j] = (T)r[j];
     }
 }
 
@@ -84,6 +87,31 @@ __device__ __forceinline__ unsigned wdg_wave_umax(unsigned v) {
     v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x140, 0xF, 0xF, true));    // row_mirror
     return max(max((unsigned)__builtin_amdgcn_readlane((int)v, 0), (unsigned)__builtin_amdgcn_readlane((int)v, 16)),
                max((unsigned)__builtin_amdgcn_readlane((int)v, 32), (unsigned)__builtin_amdgcn_readlane((int)v, 48)));
+}
+// the same for sums of doubles
+template <int CTRL>
+__device__ __forceinline__ double wdg_aw_dpp(double v) {
+    typedef int i32x2 __attribute__((ext_vector_type(2)));
+    const i32x2 b = __builtin_bit_cast(i32x2, v);
+    i32x2 r;
+    r.x = __builtin_amdgcn_update_dpp(0, b.x, CTRL, 0xF, 0xF, true);
+    r.y = __builtin_amdgcn_update_dpp(0, b.y, CTRL, 0xF, 0xF, true);
+    return __builtin_bit_cast(double, r);
+}
+__device__ __forceinline__ double wdg_aw_lane(double v, int lane) {
+    typedef int i32x2 __attribute__((ext_vector_type(2)));
+    const i32x2 b = __builtin_bit_cast(i32x2, v);
+    i32x2 r;
+    r.x = __builtin_amdgcn_readlane(b.x, lane);
+    r.y = __builtin_amdgcn_readlane(b.y, lane);
+    return __builtin_bit_cast(double, r);
+}
+__device__ __forceinline__ double wdg_aw_wave_sum(double v) {
+    v += wdg_aw_dpp<0xB1>(v);
+    v += wdg_aw_dpp<0x4E>(v);
+    v += wdg_aw_dpp<0x141>(v);
+    v += wdg_aw_dpp<0x140>(v);
+    return (wdg_aw_lane(v, 0) + wdg_aw_lane(v, 16)) + (wdg_aw_lane(v, 32) + wdg_aw_lane(v, 48));
 }
 // A block's scale from the largest bit pattern of its magnitudes (as integers: above infinity come the NaNs, which a float maximum would
 // drop).  inv = 1 / scale, 0 where the block holds zeros alone; a block that is not finite gets a NaN for its scale.
@@ -102,13 +130,11 @@ __device__ __forceinline__ float wdg_aw_scale(unsigned bits, float& inv) {
 }
 
 // clipping: the gradients' factor grad_scale c, the same bits in every workgroup (all add the same numbers in the same order); false
-// where the norm is not finite.  All threads call it.
-__device__ __forceinline__ bool wdg_aw_clip(const WdgAdamwHyper& h, double* red, float& gs) {
+// where the norm is not finite.  All threads of the workgroup call it once.  `part`: this thread's partial sum, asked for at the start.
+__device__ __forceinline__ bool wdg_aw_clip(const WdgAdamwHyper& h, double part, double* red, float& gs) {
     gs = (float)h.grad_scale;
     if (!h.parts) return true;
-    double s = 0.0;
-    for (int i = threadIdx.x; i < h.nparts; i += 256) s += h.parts[i];
-    s = wdg_wave_sum_d(s);
+    const double s = wdg_aw_wave_sum(part);
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
     __syncthreads();
     const double norm = h.grad_scale * sqrt((red[0] + red[1]) + (red[2] + red[3]));
@@ -118,36 +144,43 @@ __device__ __forceinline__ bool wdg_aw_clip(const WdgAdamwHyper& h, double* red,
     return true;
 }
 
-// One chunk.  FULL: all 4096 elements are there, so every request is issued without a condition, those of UN quads per thread before
-// the first of them is used; else the tensor ends inside, and each quad looks at what is left.
-template <int BITS, class PT, class GT, bool FULL>
-__device__ __forceinline__ void wdg_aw_chunk(const WdgAdamwChunk& q, const WdgAdamwHyper& h, float gs, float lr_bc1, float rbc2) {
-    constexpr int UN = !FULL ? 1 : BITS == 32 ? 2 : 4;
+// One chunk.  FULL: all its elements are there, so every request is issued without a condition and before the first answer is used;
+// else the tensor ends inside, and a thread takes one quad after the other and looks at what is left.  The first requests go out before the
+// workgroup adds up the norm.
+template <int BITS, int CHUNK, bool STREAM, class PT, class GT, bool FULL>
+__device__ __forceinline__ void wdg_aw_chunk(const WdgAdamwChunk& q, const WdgAdamwHyper& h, double part, double* red, float lr_bc1, float rbc2) {
+    constexpr int QUADS = CHUNK / 1024, UN = FULL ? QUADS : 1;
     const float keep = 1.f - h.lr_wd * q.decay;
     PT* p = static_cast<PT*>(q.p);
     const GT* g = static_cast<const GT*>(q.g);
     const int lane = threadIdx.x & 63;
-#pragma unroll 1
-    for (int i = 0; i < AW_CHUNK / 1024; i += UN) {
-        if (!FULL && i * 1024 + ((int)threadIdx.x & ~63) * 4 >= q.n) break;       // (the wave's whole block lies behind the tensor)
-        f32x4 w[UN], gr[UN], m[UN], v[UN];
-        unsigned cm[UN], cv[UN];
-        float sm[UN], sv[UN];
+    f32x4 w[UN], gr[UN], m[UN], v[UN];
+    unsigned cm[UN], cv[UN];
+    float sm[UN], sv[UN], gs;
+    auto behind = [&](int i) { return !FULL && i * 1024 + ((int)threadIdx.x & ~63) * 4 >= q.n; };      // (the wave's whole block lies behind the tensor)
+    auto fetch = [&](int i) {
+        if (behind(i)) return;
 #pragma unroll
         for (int k = 0; k < UN; ++k) {
             const int e = ((i + k) * 256 + (int)threadIdx.x) * 4, n = FULL ? 4 : q.n - e;      // (n: elements from here on, maybe none)
-            w[k] = wdg_aw_load(p + e, n);
-            gr[k] = wdg_aw_load(g + e, n);
+            w[k] = wdg_aw_load<STREAM>(p + e, n);
+            gr[k] = wdg_aw_load<STREAM>(g + e, n);
             if constexpr (BITS == 32) {
-                m[k] = wdg_aw_load(static_cast<const float*>(q.m) + e, n);
-                v[k] = wdg_aw_load(static_cast<const float*>(q.v) + e, n);
+                m[k] = wdg_aw_load<STREAM>(static_cast<const float*>(q.m) + e, n);
+                v[k] = wdg_aw_load<STREAM>(static_cast<const float*>(q.v) + e, n);
             } else {
-                cm[k] = static_cast<const unsigned*>(q.m)[e >> 2];
-                cv[k] = static_cast<const unsigned*>(q.v)[e >> 2];
-                sm[k] = q.ms[e / AW_BLOCK];
-                sv[k] = q.vs[e / AW_BLOCK];
+                cm[k] = wdg_vec_load<unsigned, 1, STREAM>(static_cast<const unsigned*>(q.m) + (e >> 2)).e[0];
+                cv[k] = wdg_vec_load<unsigned, 1, STREAM>(static_cast<const unsigned*>(q.v) + (e >> 2)).e[0];
+                sm[k] = ((const WDG_GLOBAL float*)q.ms)[e / AW_BLOCK];
+                sv[k] = ((const WDG_GLOBAL float*)q.vs)[e / AW_BLOCK];
             }
         }
+    };
+    fetch(0);
+    if (!wdg_aw_clip(h, part, red, gs)) return;
+#pragma unroll 1
+    for (int i = 0;; fetch(i)) {
+        if (behind(i)) return;
 #pragma unroll
         for (int k = 0; k < UN; ++k) {
             const int e = ((i + k) * 256 + (int)threadIdx.x) * 4, n = FULL ? 4 : q.n - e;
@@ -172,12 +205,12 @@ __device__ __forceinline__ void wdg_aw_chunk(const WdgAdamwChunk& q, const WdgAd
                     tv = max(tv, j < n ? __builtin_bit_cast(unsigned, b) & 0x7fffffffu : 0u);
                 }
             }
-            wdg_aw_store(p + e, n, w[k]);
-            if (q.copy_type == WDG_BF16) wdg_aw_store(static_cast<__bf16*>(q.copy) + e, n, w[k]);
-            else if (q.copy_type == WDG_F16) wdg_aw_store(static_cast<_Float16*>(q.copy) + e, n, w[k]);
+            wdg_aw_store<STREAM>(p + e, n, w[k]);
+            if (q.copy_type == WDG_BF16) wdg_aw_store<STREAM>(static_cast<__bf16*>(q.copy) + e, n, w[k]);
+            else if (q.copy_type == WDG_F16) wdg_aw_store<STREAM>(static_cast<_Float16*>(q.copy) + e, n, w[k]);
             if constexpr (BITS == 32) {
-                wdg_aw_store(static_cast<float*>(q.m) + e, n, m[k]);
-                wdg_aw_store(static_cast<float*>(q.v) + e, n, v[k]);
+                wdg_aw_store<STREAM>(static_cast<float*>(q.m) + e, n, m[k]);
+                wdg_aw_store<STREAM>(static_cast<float*>(q.v) + e, n, v[k]);
             } else {
                 float im, iv;
                 const float nm = wdg_aw_scale(wdg_wave_umax(tm), im), nv = wdg_aw_scale(wdg_wave_umax(tv), iv);
@@ -193,79 +226,92 @@ __device__ __forceinline__ void wdg_aw_chunk(const WdgAdamwChunk& q, const WdgAd
                     om |= ((unsigned)ai & 255u) << (8 * j);
                     ov |= ((unsigned)bi & 255u) << (8 * j);
                 }
-                static_cast<unsigned*>(q.m)[e >> 2] = om;
-                static_cast<unsigned*>(q.v)[e >> 2] = ov;
+                wdg_vec_store<unsigned, 1, STREAM>(static_cast<unsigned*>(q.m) + (e >> 2), {{om}});
+                wdg_vec_store<unsigned, 1, STREAM>(static_cast<unsigned*>(q.v) + (e >> 2), {{ov}});
                 if (lane == 0) {
-                    q.ms[e / AW_BLOCK] = nm;
-                    q.vs[e / AW_BLOCK] = nv;
+                    ((WDG_GLOBAL float*)q.ms)[e / AW_BLOCK] = nm;
+                    ((WDG_GLOBAL float*)q.vs)[e / AW_BLOCK] = nv;
                 }
             }
         }
+        i += UN;
+        if (i >= QUADS) return;
     }
 }
 
-template <int BITS, class PT, class GT>
-__device__ __forceinline__ void wdg_aw_by_size(const WdgAdamwChunk& q, const WdgAdamwHyper& h, float gs, float lr_bc1, float rbc2) {
-    if (q.n == AW_CHUNK) wdg_aw_chunk<BITS, PT, GT, true>(q, h, gs, lr_bc1, rbc2);
-    else wdg_aw_chunk<BITS, PT, GT, false>(q, h, gs, lr_bc1, rbc2);
+template <int BITS, int CHUNK, bool STREAM, class PT, class GT>
+__device__ __forceinline__ void wdg_aw_by_size(const WdgAdamwChunk& q, const WdgAdamwHyper& h, double part, double* red, float lr_bc1, float rbc2) {
+    if (q.n == CHUNK) wdg_aw_chunk<BITS, CHUNK, STREAM, PT, GT, true>(q, h, part, red, lr_bc1, rbc2);
+    else wdg_aw_chunk<BITS, CHUNK, STREAM, PT, GT, false>(q, h, part, red, lr_bc1, rbc2);
 }
-template <int BITS, class PT>
-__device__ __forceinline__ void wdg_aw_by_grad(const WdgAdamwChunk& q, const WdgAdamwHyper& h, float gs, float lr_bc1, float rbc2) {
-    if (q.g_type == WDG_F32) wdg_aw_by_size<BITS, PT, float>(q, h, gs, lr_bc1, rbc2);
-    else if (q.g_type == WDG_BF16) wdg_aw_by_size<BITS, PT, __bf16>(q, h, gs, lr_bc1, rbc2);
-    else wdg_aw_by_size<BITS, PT, _Float16>(q, h, gs, lr_bc1, rbc2);
+template <int BITS, int CHUNK, bool STREAM, class PT>
+__device__ __forceinline__ void wdg_aw_by_grad(const WdgAdamwChunk& q, const WdgAdamwHyper& h, double part, double* red, float lr_bc1, float rbc2) {
+    if (q.g_type == WDG_F32) wdg_aw_by_size<BITS, CHUNK, STREAM, PT, float>(q, h, part, red, lr_bc1, rbc2);
+    else if (q.g_type == WDG_BF16) wdg_aw_by_size<BITS, CHUNK, STREAM, PT, __bf16>(q, h, part, red, lr_bc1, rbc2);
+    else wdg_aw_by_size<BITS, CHUNK, STREAM, PT, _Float16>(q, h, part, red, lr_bc1, rbc2);
 }
 
-template <int BITS>
+template <int BITS, int CHUNK, bool STREAM>
 __global__ void __launch_bounds__(256) wdg_adamw_kernel(const WdgAdamwChunk* __restrict__ table, const WdgAdamwHyper h) {
     __shared__ double red[4];
+    const double part = h.parts && (int)threadIdx.x < h.nparts ? h.parts[threadIdx.x] : 0.0;
     const WdgAdamwChunk q = table[blockIdx.x];
-    float gs, lr_bc1 = h.lr_bc1, rbc2 = h.rbc2;
+    float lr_bc1 = h.lr_bc1, rbc2 = h.rbc2;
     if (h.step_dev) {
         // 1 - beta^t = -expm1(t log beta): the difference keeps its digits when beta^t is close to 1
         const double t = (double)*h.step_dev;
         lr_bc1 = h.lr / -expm1f((float)(t * h.log_b1));
         rbc2 = 1.f / sqrtf(-expm1f((float)(t * h.log_b2)));
     }
-    if (!wdg_aw_clip(h, red, gs)) return;
-    if (q.p_type == WDG_F32) wdg_aw_by_grad<BITS, float>(q, h, gs, lr_bc1, rbc2);
-    else if (q.p_type == WDG_BF16) wdg_aw_by_grad<BITS, __bf16>(q, h, gs, lr_bc1, rbc2);
-    else wdg_aw_by_grad<BITS, _Float16>(q, h, gs, lr_bc1, rbc2);
+    if (q.p_type == WDG_F32) wdg_aw_by_grad<BITS, CHUNK, STREAM, float>(q, h, part, red, lr_bc1, rbc2);
+    else if (q.p_type == WDG_BF16) wdg_aw_by_grad<BITS, CHUNK, STREAM, __bf16>(q, h, part, red, lr_bc1, rbc2);
+    else wdg_aw_by_grad<BITS, CHUNK, STREAM, _Float16>(q, h, part, red, lr_bc1, rbc2);
 }
 
 // ---- sum of g^2 over all chunks; fp64, since a square leaves fp32's range where the gradient itself does not -------------------------
 // Four chunks at a time per workgroup (256 threads each), as many workgroups as the chip holds: the launch reads one tensor, and what it
 // needs is requests in flight.
-template <class GT>
+template <int CHUNK, bool STREAM, class GT>
 __device__ __forceinline__ double wdg_aw_sumsq(const GT* g, int n) {
     const int t = (int)(threadIdx.x & 255) * 4;
-    f32x4 v[AW_CHUNK / 1024];
-    if (n == AW_CHUNK) {
+    f32x4 v[CHUNK / 1024];
+    if (n == CHUNK) {
 #pragma unroll
-        for (int i = 0; i < AW_CHUNK / 1024; ++i) v[i] = wdg_aw_load(g + i * 1024 + t, 4);
+        for (int i = 0; i < CHUNK / 1024; ++i) v[i] = wdg_aw_load<STREAM>(g + i * 1024 + t, 4);
     } else {
 #pragma unroll
-        for (int i = 0; i < AW_CHUNK / 1024; ++i) v[i] = wdg_aw_load(g + i * 1024 + t, n - i * 1024 - t);
+        for (int i = 0; i < CHUNK / 1024; ++i) v[i] = wdg_aw_load<STREAM>(g + i * 1024 + t, n - i * 1024 - t);
     }
     double s = 0.0;
 #pragma unroll
-    for (int i = 0; i < AW_CHUNK / 1024; ++i)
+    for (int i = 0; i < CHUNK / 1024; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) s += (double)v[i][j] * (double)v[i][j];
     return s;
 }
+template <int CHUNK, bool STREAM>
 __global__ void __launch_bounds__(1024) wdg_adamw_sumsq_kernel(const WdgAdamwChunk* __restrict__ table, int chunks, double* parts) {
+    constexpr int R = AW_CHUNK / CHUNK;                   // records at a time
     __shared__ double red[16];
     double s = 0.0;
-    for (int c = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 8); c < chunks; c += gridDim.x * 4) {
-        const void* g = table[c].g;
-        const int n = table[c].n;
-        const unsigned char type = table[c].g_type;
-        if (type == WDG_F32) s += wdg_aw_sumsq(static_cast<const float*>(g), n);
-        else if (type == WDG_BF16) s += wdg_aw_sumsq(static_cast<const __bf16*>(g), n);
-        else s += wdg_aw_sumsq(static_cast<const _Float16*>(g), n);
+    for (int c0 = (blockIdx.x * 4 + __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 8)) * R; c0 < chunks; c0 += gridDim.x * (4 * R)) {
+        const void* g[R];
+        int n[R], type[R];
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const WdgAdamwChunk& q = table[min(c0 + r, chunks - 1)];
+            g[r] = q.g;
+            n[r] = c0 + r < chunks ? q.n : 0;
+            type[r] = q.g_type;
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            if (type[r] == WDG_F32) s += wdg_aw_sumsq<CHUNK, STREAM>(static_cast<const float*>(g[r]), n[r]);
+            else if (type[r] == WDG_BF16) s += wdg_aw_sumsq<CHUNK, STREAM>(static_cast<const __bf16*>(g[r]), n[r]);
+            else s += wdg_aw_sumsq<CHUNK, STREAM>(static_cast<const _Float16*>(g[r]), n[r]);
+        }
     }
-    s = wdg_wave_sum_d(s);
+    s = wdg_aw_wave_sum(s);
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
     __syncthreads();
     if (threadIdx.x == 0) {
@@ -279,7 +325,7 @@ __global__ void __launch_bounds__(256) wdg_adamw_norm_kernel(const double* __res
     __shared__ double red[4];
     double s = 0.0;
     for (int i = threadIdx.x; i < nparts; i += 256) s += parts[i];
-    s = wdg_wave_sum_d(s);
+    s = wdg_aw_wave_sum(s);
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
     __syncthreads();
     if (threadIdx.x == 0) norm[0] = (float)(scale * sqrt((red[0] + red[1]) + (red[2] + red[3])));
@@ -327,6 +373,20 @@ static const char* aw_check(const wdg_adamw_tensor& t, int bits) {
     return nullptr;
 }
 
+// Lists of fewer than 4096 chunks of 4096 (16 M elements) in chunks of 1024: more workgroups than the chip holds at once, and one request
+// per tensor and thread, hide a chunk's latency better (us of an unclipped fp32 step with 1024 / 4096, 32-bit states: 0.2 M elements
+// 3.5 / 4.6, 2 M 10.5 / 13.8, 8 M 43.7 / 45.7; 8-bit: 3.8 / 6.4, 9.5 / 13.0, 23 / 27).  Above, the table and the norm that every workgroup
+// of a clipped step adds up cost what that gains (16 M, 8-bit, clipped: 68 / 66).
+static int aw_chunk_size(int64_t chunks) { return chunks < 4096 ? AW_SMALL : AW_CHUNK; }
+
+// A step whose tensors leave no room in the chip's last-level cache (256 MiB) is streamed past it: nothing of it would be there at the
+// next step.  us without / with, 32-bit states: 8 M fp32 (122 MiB) 43 / 38, 16 M 86 / 74, 128 M 681 / 627; 8-bit: 16 M (152 MiB) 50 / 45,
+// 128 M 383 / 351; smaller ones stay: 4 M (61 MiB) 18.5 / 20.4.
+static bool aw_stream_step(const wdg_adamw_batch* b) { return b->bytes >= 96ll << 20; }
+// The norm's pass leaves the gradients in the cache for the step where they fit: 32 M fp32 (122 MiB), clipped, 178 us with streaming and
+// 159 without; 128 M (488 MiB) 703 and 792.
+static bool aw_stream_norm(const wdg_adamw_batch* b) { return b->grad_bytes >= 192ll << 20; }
+
 struct AwRange {
     uintptr_t begin, end;
     bool written;
@@ -334,7 +394,7 @@ struct AwRange {
 
 static int aw_create(wdg_adamw_batch** out, const wdg_adamw_tensor* tensors, int n, int bits) {
     std::vector<AwRange> ranges;
-    int64_t chunks = 0;
+    int64_t chunks = 0, total = 0, grads = 0;
     for (int i = 0; i < n; ++i) {
         const wdg_adamw_tensor& t = tensors[i];
         if (const char* why = aw_check(t, bits)) {
@@ -345,9 +405,11 @@ static int aw_create(wdg_adamw_batch** out, const wdg_adamw_tensor* tensors, int
         const int64_t blocks = (t.n + AW_BLOCK - 1) / AW_BLOCK;
         auto add = [&](const void* p, int64_t bytes, bool written) {
             if (p) ranges.push_back({(uintptr_t)p, (uintptr_t)p + (uintptr_t)bytes, written});
+            if (p) total += bytes;
         };
         add(t.p, t.n * aw_bytes(t.p_type), true);
         add(t.g, t.n * aw_bytes(t.g_type), false);
+        grads += t.n * aw_bytes(t.g_type);
         add(t.copy, t.n * 2, true);
         add(t.m, bits == 8 ? blocks * AW_BLOCK : t.n * 4, true);
         add(t.v, bits == 8 ? blocks * AW_BLOCK : t.n * 4, true);
@@ -374,15 +436,18 @@ static int aw_create(wdg_adamw_batch** out, const wdg_adamw_tensor* tensors, int
     }
     wdg_adamw_batch* b = new wdg_adamw_batch();
     b->bits = bits;
+    b->chunk = aw_chunk_size(chunks);
+    b->bytes = total;
+    b->grad_bytes = grads;
     try {
-        b->chunks.reserve((size_t)chunks);
+        b->chunks.reserve((size_t)(chunks * (AW_CHUNK / b->chunk)));
     } catch (...) {
         delete b;
         throw;
     }
     for (int i = 0; i < n; ++i) {
         const wdg_adamw_tensor& t = tensors[i];
-        for (int64_t e = 0; e < t.n; e += AW_CHUNK) {
+        for (int64_t e = 0; e < t.n; e += b->chunk) {
             WdgAdamwChunk q;
             memset(&q, 0, sizeof(q));
             q.p = (char*)t.p + e * aw_bytes(t.p_type);
@@ -392,7 +457,7 @@ static int aw_create(wdg_adamw_batch** out, const wdg_adamw_tensor* tensors, int
             q.ms = bits == 8 ? t.m_scale + e / AW_BLOCK : nullptr;
             q.vs = bits == 8 ? t.v_scale + e / AW_BLOCK : nullptr;
             q.copy = t.copy ? (char*)t.copy + e * 2 : nullptr;
-            q.n = (int)std::min<int64_t>(AW_CHUNK, t.n - e);
+            q.n = (int)std::min<int64_t>(b->chunk, t.n - e);
             q.p_type = (unsigned char)t.p_type;
             q.g_type = (unsigned char)t.g_type;
             q.copy_type = t.copy ? (unsigned char)t.copy_type : 0;
@@ -434,11 +499,16 @@ extern "C" int wdg_adamw_destroy(wdg_adamw_batch* b) {
 
 extern "C" size_t wdg_adamw_scratch_bytes(void) { return AW_PARTS * sizeof(double); }
 
-static int aw_parts(const wdg_adamw_batch* b) { return (int)std::min<size_t>(AW_PARTS, (b->chunks.size() + 3) / 4); }
+static int aw_parts(const wdg_adamw_batch* b) {
+    const size_t each = 4 * (AW_CHUNK / b->chunk);        // chunks that a workgroup takes at a time
+    return (int)std::min<size_t>(AW_PARTS, (b->chunks.size() + each - 1) / each);
+}
 
 static int aw_sumsq(const wdg_adamw_batch* b, double* parts, hipStream_t st) {
     if (aw_parts(b) == 0) return WDG_OK;
-    hipLaunchKernelGGL(wdg_adamw_sumsq_kernel, dim3(aw_parts(b)), dim3(1024), 0, st, b->table, (int)b->chunks.size(), parts);
+    const auto kernel = b->chunk == AW_SMALL ? wdg_adamw_sumsq_kernel<AW_SMALL, false>
+                        : aw_stream_norm(b) ? wdg_adamw_sumsq_kernel<AW_CHUNK, true> : wdg_adamw_sumsq_kernel<AW_CHUNK, false>;
+    hipLaunchKernelGGL(kernel, dim3(aw_parts(b)), dim3(1024), 0, st, b->table, (int)b->chunks.size(), parts);
     WDG_LAUNCH_CHECK();
     return WDG_OK;
 }
@@ -460,6 +530,12 @@ extern "C" int wdg_adamw_grad_norm(const wdg_adamw_batch* b, double grad_scale, 
     }
     const int rc = aw_sumsq(b, (double*)scratch, (hipStream_t)stream);
     return rc != WDG_OK ? rc : aw_norm(b, grad_scale, norm, (const double*)scratch, (hipStream_t)stream);
+}
+
+template <int BITS>
+static auto aw_step_kernel(const wdg_adamw_batch* b) {
+    if (b->chunk == AW_SMALL) return aw_stream_step(b) ? wdg_adamw_kernel<BITS, AW_SMALL, true> : wdg_adamw_kernel<BITS, AW_SMALL, false>;
+    return aw_stream_step(b) ? wdg_adamw_kernel<BITS, AW_CHUNK, true> : wdg_adamw_kernel<BITS, AW_CHUNK, false>;
 }
 
 extern "C" int wdg_adamw_step(const wdg_adamw_batch* b, const wdg_adamw_args* a, void* scratch, size_t scratch_bytes, wdg_stream stream) {
@@ -505,8 +581,8 @@ extern "C" int wdg_adamw_step(const wdg_adamw_batch* b, const wdg_adamw_args* a,
         h.norm = a->norm;
     }
     const dim3 grid((unsigned)b->chunks.size());
-    if (b->bits == 32) hipLaunchKernelGGL(wdg_adamw_kernel<32>, grid, dim3(256), 0, st, b->table, h);
-    else hipLaunchKernelGGL(wdg_adamw_kernel<8>, grid, dim3(256), 0, st, b->table, h);
+    const auto kernel = b->bits == 32 ? aw_step_kernel<32>(b) : aw_step_kernel<8>(b);
+    hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, b->table, h);
     WDG_LAUNCH_CHECK();
     return WDG_OK;
 }

@@ -102,7 +102,7 @@ __device__ __forceinline__ void wdg_ln_row_sums(float (&v)[U], float* red) {
     }
 }
 
-template <class T, int V, int K, int L, int NT, int U, bool TAIL>
+template <class T, int V, int K, int L, int NT, int U, bool TAIL, bool STREAM>
 __global__ void __launch_bounds__(NT) wdg_layernorm_fwd_kernel(const T* x, int64_t ldx, const void* __restrict__ gamma,
                                                                const void* __restrict__ beta, int ptype, float eps, T* z, int64_t ldz,
                                                                float* mean_rstd, int64_t P, int C) {
@@ -124,7 +124,7 @@ __global__ void __launch_bounds__(NT) wdg_layernorm_fwd_kernel(const T* x, int64
         for (int u = 0; u < U; ++u) {
             const int64_t p = std::min<int64_t>(p0 + u * RG + g, P - 1);
 #pragma unroll
-            for (int k = 0; k < K; ++k) ahead[u][k] = wdg_vec_load<T, V>(x + p * ldx + at.col[k]);
+            for (int k = 0; k < K; ++k) ahead[u][k] = wdg_vec_load<T, V, STREAM>(x + p * ldx + at.col[k]);
         }
     };
     fetch((int64_t)blockIdx.x * (RG * U));
@@ -173,7 +173,7 @@ __global__ void __launch_bounds__(NT) wdg_layernorm_fwd_kernel(const T* x, int64
                     WdgVec<T, V> r;
 #pragma unroll
                     for (int j = 0; j < V; ++j) r.e[j] = (T)fmaf(fmaf((float)xv[u][k].e[j] - s[u], rstd, shift), gm[k][j], bt[k][j]);
-                    if (!TAIL || at.dup[k] < V) wdg_vec_store<T, V>(z + p * ldz + at.col[k], r);
+                    if (!TAIL || at.dup[k] < V) wdg_vec_store<T, V, STREAM>(z + p * ldz + at.col[k], r);
                 }
                 if (mean_rstd && sub == 0) {
                     mean_rstd[2 * p] = s[u] + corr;
@@ -185,7 +185,7 @@ __global__ void __launch_bounds__(NT) wdg_layernorm_fwd_kernel(const T* x, int64
 }
 
 // part: NULL, or one row [dgamma | dbeta] (each of C rounded up to 4) of partial sums per workgroup
-template <class T, int V, int K, int L, int NT, int U, bool TAIL>
+template <class T, int V, int K, int L, int NT, int U, bool TAIL, bool STREAM>
 __global__ void __launch_bounds__(NT) wdg_layernorm_bwd_kernel(const T* dz, int64_t lddz, const T* x, int64_t ldx,
                                                                const float* __restrict__ mean_rstd, const void* __restrict__ gamma, int ptype,
                                                                T* dx, int64_t lddx, float* part, int64_t P, int C) {
@@ -215,8 +215,8 @@ __global__ void __launch_bounds__(NT) wdg_layernorm_bwd_kernel(const T* dz, int6
             rstd_a[u] = mean_rstd[2 * p + 1];
 #pragma unroll
             for (int k = 0; k < K; ++k) {
-                x_a[u][k] = wdg_vec_load<T, V>(x + p * ldx + at.col[k]);
-                g_a[u][k] = wdg_vec_load<T, V>(dz + p * lddz + at.col[k]);
+                x_a[u][k] = wdg_vec_load<T, V, STREAM>(x + p * ldx + at.col[k]);
+                g_a[u][k] = wdg_vec_load<T, V, STREAM>(dz + p * lddz + at.col[k]);
             }
         }
     };
@@ -268,7 +268,7 @@ __global__ void __launch_bounds__(NT) wdg_layernorm_bwd_kernel(const T* dz, int6
                         const float xh = ((float)xv[u][k].e[j] - mean[u]) * rstd[u];
                         r.e[j] = (T)(rstd[u] * ((float)gv[u][k].e[j] * gm[k][j] - m1 - xh * m2));
                     }
-                    if (!TAIL || at.dup[k] < V) wdg_vec_store<T, V>(dx + p * lddx + at.col[k], r);
+                    if (!TAIL || at.dup[k] < V) wdg_vec_store<T, V, STREAM>(dx + p * lddx + at.col[k], r);
                 }
             }
         }
@@ -579,6 +579,12 @@ static bool ln_dispatch(const LnGeom& g, F& f) {
     return true;
 }
 
+// Tensors that together pass the chip's last-level cache (256 MiB) are streamed past it.  us without / with: 16384 x 4096 fp32 forward
+// 97 / 92, backward 153 / 138; 16384 x 8192 bf16 97 / 89, 154 / 142; 65536 x 1024 bf16 backward 80 / 73.  Below that size the tensors may
+// still be there from the launch before, and stay for the one behind (512 x 4096 bf16 9.4 / 9.9); rows that are not whole vectors of all
+// lanes gain nothing (16384 x 10000 bf16 backward 207 / 210).
+static bool ln_stream(int64_t bytes) { return bytes >= 256ll << 20; }
+
 static bool ln_types_ok(int type, int ptype) {
     return type >= WDG_F32 && type <= WDG_F16 && (ptype == WDG_F32 || ptype == type);
 }
@@ -600,10 +606,11 @@ struct LnFwd {
     LnGeom g;
     template <int V, int K, int L, int NT, int U>
     void run() {
-        if (C == (int64_t)V * K * (L ? L : g.NT))
-            hipLaunchKernelGGL((wdg_layernorm_fwd_kernel<T, V, K, L, NT, U, false>), dim3(g.blocks), dim3(g.NT), 0, st, x, ldx, gamma, beta, ptype, eps, z, ldz, mean_rstd, P, (int)C);
-        else
-            hipLaunchKernelGGL((wdg_layernorm_fwd_kernel<T, V, K, L, NT, U, true>), dim3(g.blocks), dim3(g.NT), 0, st, x, ldx, gamma, beta, ptype, eps, z, ldz, mean_rstd, P, (int)C);
+        const bool whole = C == (int64_t)V * K * (L ? L : g.NT);
+        const auto kernel = !whole ? wdg_layernorm_fwd_kernel<T, V, K, L, NT, U, true, false>
+                            : ln_stream(2 * P * C * sizeof(T)) ? wdg_layernorm_fwd_kernel<T, V, K, L, NT, U, false, true>
+                                                                : wdg_layernorm_fwd_kernel<T, V, K, L, NT, U, false, false>;
+        hipLaunchKernelGGL(kernel, dim3(g.blocks), dim3(g.NT), 0, st, x, ldx, gamma, beta, ptype, eps, z, ldz, mean_rstd, P, (int)C);
     }
 };
 
@@ -665,10 +672,11 @@ struct LnBwd {
     LnGeom g;
     template <int V, int K, int L, int NT, int U>
     void run() {
-        if (C == (int64_t)V * K * (L ? L : g.NT))
-            hipLaunchKernelGGL((wdg_layernorm_bwd_kernel<T, V, K, L, NT, U, false>), dim3(g.blocks), dim3(g.NT), 0, st, dz, lddz, x, ldx, mean_rstd, gamma, ptype, dx, lddx, part, P, (int)C);
-        else
-            hipLaunchKernelGGL((wdg_layernorm_bwd_kernel<T, V, K, L, NT, U, true>), dim3(g.blocks), dim3(g.NT), 0, st, dz, lddz, x, ldx, mean_rstd, gamma, ptype, dx, lddx, part, P, (int)C);
+        const bool whole = C == (int64_t)V * K * (L ? L : g.NT);
+        const auto kernel = !whole ? wdg_layernorm_bwd_kernel<T, V, K, L, NT, U, true, false>
+                            : ln_stream(3 * P * C * sizeof(T)) ? wdg_layernorm_bwd_kernel<T, V, K, L, NT, U, false, true>
+                                                                : wdg_layernorm_bwd_kernel<T, V, K, L, NT, U, false, false>;
+        hipLaunchKernelGGL(kernel, dim3(g.blocks), dim3(g.NT), 0, st, dz, lddz, x, ldx, mean_rstd, gamma, ptype, dx, lddx, part, P, (int)C);
     }
 };
 
