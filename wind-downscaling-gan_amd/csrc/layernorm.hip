@@ -336,6 +336,14 @@ __device__ __forceinline__ void wdg_ln_row(const T* x, int64_t C, F&& f) {
         }
     }
 }
+// the parameters beside n elements from column c on
+template <class T, int V>
+__device__ __forceinline__ void wdg_ln_params_of(float (&r)[V], const void* p, int ptype, int64_t c, int n, float none) {
+    if (n == V) wdg_ln_params<T, V>(r, p, ptype, c, none);
+    else
+#pragma unroll
+        for (int j = 0; j < V; ++j) r[j] = wdg_ln_param<T>(p, ptype, j < n ? c + j : c, none);
+}
 template <class T, int V>
 __device__ __forceinline__ void wdg_ln_put(T* p, int n, const WdgVec<T, V>& v) {
     if (n == V) wdg_vec_store<T, V>(p, v);
@@ -375,11 +383,11 @@ __global__ void __launch_bounds__(LNW_NT) wdg_layernorm_fwd_wide_kernel(const T*
         const float rstd = 1.f / sqrtf(var + eps);
         wdg_ln_row<T, V>(xr, C, [&](int64_t c, int n, const WdgVec<T, V>& v) {
             WdgVec<T, V> r;
+            float gm[V], bt[V];
+            wdg_ln_params_of<T, V>(gm, gamma, ptype, c, n, 1.f);
+            wdg_ln_params_of<T, V>(bt, beta, ptype, c, n, 0.f);
 #pragma unroll
-            for (int j = 0; j < V; ++j) {
-                const int64_t cc = j < n ? c + j : c;
-                r.e[j] = (T)((((float)v.e[j] - mean0) - corr) * rstd * wdg_ln_param<T>(gamma, ptype, cc, 1.f) + wdg_ln_param<T>(beta, ptype, cc, 0.f));
-            }
+            for (int j = 0; j < V; ++j) r.e[j] = (T)((((float)v.e[j] - mean0) - corr) * rstd * gm[j] + bt[j]);
             wdg_ln_put<T, V>(zr + c, n, r);
         });
         if (mean_rstd && threadIdx.x == 0) {
@@ -411,10 +419,12 @@ __global__ void __launch_bounds__(LNW_NT) wdg_layernorm_bwd_wide_kernel(const T*
         };
         wdg_ln_row<T, V>(gr, C, [&](int64_t c, int n, const WdgVec<T, V>& g) {
             const WdgVec<T, V> u = other(c, n);
+            float gm[V];
+            wdg_ln_params_of<T, V>(gm, gamma, ptype, c, n, 1.f);
 #pragma unroll
             for (int j = 0; j < V; ++j)
                 if (j < n) {
-                    const float a = (float)g.e[j] * wdg_ln_param<T>(gamma, ptype, c + j, 1.f);
+                    const float a = (float)g.e[j] * gm[j];
                     s1 += a;
                     s2 += a * (((float)u.e[j] - mean) * rstd);
                 }
@@ -424,9 +434,11 @@ __global__ void __launch_bounds__(LNW_NT) wdg_layernorm_bwd_wide_kernel(const T*
         wdg_ln_row<T, V>(gr, C, [&](int64_t c, int n, const WdgVec<T, V>& g) {
             const WdgVec<T, V> u = other(c, n);
             WdgVec<T, V> r;
+            float gm[V];
+            wdg_ln_params_of<T, V>(gm, gamma, ptype, c, n, 1.f);
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-                const float a = (float)g.e[j] * wdg_ln_param<T>(gamma, ptype, j < n ? c + j : c, 1.f);
+                const float a = (float)g.e[j] * gm[j];
                 r.e[j] = (T)(rstd * (a - s1 - ((float)u.e[j] - mean) * rstd * s2));
             }
             wdg_ln_put<T, V>(dr + c, n, r);
@@ -435,33 +447,47 @@ __global__ void __launch_bounds__(LNW_NT) wdg_layernorm_bwd_wide_kernel(const T*
 }
 
 // ---- parameter gradients -----------------------------------------------------------------------------------------------------------
-// Partial sums [slice][dgamma | dbeta][C, rounded up to 4]: a block owns 256 V columns of one slice of the rows.
+// Partial sums [slice][dgamma | dbeta][C, rounded up to 4]: a block owns 256 V columns of one slice of the rows (C >= V; the last vector
+// reaches back over columns of its neighbour, whose sums it does not store).
 template <class T, int V>
 __global__ void __launch_bounds__(256) wdg_layernorm_colsum_kernel(const T* __restrict__ dz, int64_t lddz, const T* __restrict__ x,
                                                                    int64_t ldx, const float* __restrict__ mean_rstd, float* part,
                                                                    int64_t P, int64_t C, int slices) {
-    const int64_t c = ((int64_t)blockIdx.x * 256 + threadIdx.x) * V;
-    if (c >= C) return;
-    const int n = (int)std::min<int64_t>(V, C - c);
+    const int64_t c0 = ((int64_t)blockIdx.x * 256 + threadIdx.x) * V;
+    if (c0 >= C) return;
+    const int64_t c = std::min<int64_t>(c0, C - V);
     const int64_t per = (P + slices - 1) / slices, p0 = blockIdx.y * per, p1 = std::min<int64_t>(P, p0 + per);
     float sg[V], sb[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) sg[j] = sb[j] = 0.f;
-    for (int64_t p = p0; p < p1; ++p) {
-        const float mean = mean_rstd[2 * p], rstd = mean_rstd[2 * p + 1];
+    constexpr int U = 4;
+    for (int64_t p = p0; p < p1; p += U) {
+        WdgVec<T, V> xv[U], gv[U];
+        float mean[U], rstd[U];
 #pragma unroll
-        for (int j = 0; j < V; ++j)
-            if (j < n) {
-                const float g = (float)dz[p * lddz + c + j];
-                sg[j] += g * (((float)x[p * ldx + c + j] - mean) * rstd);
+        for (int u = 0; u < U; ++u) {
+            const int64_t q = std::min<int64_t>(p + u, P - 1);
+            mean[u] = mean_rstd[2 * q];
+            rstd[u] = mean_rstd[2 * q + 1];
+            xv[u] = wdg_vec_load<T, V>(x + q * ldx + c);
+            gv[u] = wdg_vec_load<T, V>(dz + q * lddz + c);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (p + u >= p1) break;
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const float g = (float)gv[u].e[j];
+                sg[j] += g * (((float)xv[u].e[j] - mean[u]) * rstd[u]);
                 sb[j] += g;
             }
+        }
     }
     const int64_t Cp = (C + 3) & ~3ll;
     float* row = part + (int64_t)blockIdx.y * 2 * Cp;
 #pragma unroll
     for (int j = 0; j < V; ++j)
-        if (j < n) {
+        if (c + j >= c0) {
             row[c + j] = sg[j];
             row[Cp + c + j] = sb[j];
         }
