@@ -406,7 +406,7 @@ int wdg_ln_bwd(const float* dz, int lddz, const float* y, int ldy, const float* 
  *   - statistics and sums are fp32; z and dx are rounded once.  A NaN or an infinity makes its own row what the formula makes of it,
  *     and its column of the parameter gradients.
  *   - dgamma, dbeta: fp32 [C], either may be NULL; accumulate != 0 adds to them, 0 overwrites them (with zeros when P == 0).
- *     ws: wdg_layernorm_bwd_ws_bytes() of scratch, needed with either (16-byte aligned, not shared with work that may run at the
+ *     ws: wdg_layernorm_bwd_ws_bytes() of scratch, needed with either (4-byte aligned, not shared with work that may run at the
  *     same time). */
 int wdg_layernorm_fwd(const void* x, int64_t ldx, const void* gamma, const void* beta, float eps, void* z, int64_t ldz,
                       float* mean_rstd, int64_t P, int64_t C, int type, int param_type, wdg_stream stream);

@@ -27,7 +27,8 @@ def entry(n=10, p=torch.float32, g=torch.float32, copy=None):
 @pytest.mark.parametrize("bad", [
     (torch.zeros(10, dtype=torch.float64), torch.zeros(10), 1.0), (torch.zeros(10), torch.zeros(11), 1.0), (torch.zeros(20)[::2], torch.zeros(10), 1.0),
     (torch.zeros(10), torch.zeros(20)[::2], 1.0), (torch.zeros(10), torch.zeros(10, dtype=torch.int32), 1.0), (torch.zeros(10), torch.zeros(10), 1.0, torch.zeros(10)),
-    (torch.zeros(10), torch.zeros(10), 1.0, torch.zeros(9, dtype=torch.bfloat16)), (torch.zeros(10, device="meta"), torch.zeros(10), 1.0),
+    (torch.zeros(10), torch.zeros(10), 1.0, torch.zeros(9, dtype=torch.bfloat16)), (torch.zeros(10), torch.zeros(10)), (torch.zeros(10), None, 1.0),
+    (torch.zeros(10), torch.zeros(10), torch.ones(1)), (torch.zeros(10), torch.zeros(10), 1.0, None, None), (torch.zeros(10, device="meta"), torch.zeros(10), 1.0),
 ])
 def test_list_refuses(ops, bad):
     with pytest.raises(ValueError):

@@ -163,6 +163,26 @@ def test_hyper_parameters(h, bits, hip_ops):
 
 
 @pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("h", [dict(beta1=0.0, beta2=0.0), dict(beta1=0.99, beta2=0.9999)])
+def test_step_count_in_device_memory(h, bits, hip_ops):
+    b, _ = make(hip_ops, [5000, 77], bits=bits, seed=4)
+    h = {**HYPER, **h}
+    for t in (1, 2, 100000):
+        at = torch.tensor([t], dtype=torch.int64, device="cuda")
+        step_close(b, t, h=h, call=lambda: b.step(at, **h))      # noqa: B023
+
+
+def test_large_list(hip_ops):
+    """More than 4096 chunks of 4096 elements and more than the cache holds: the other chunk size, and streamed requests."""
+    for bits, sizes, g in ((32, [17000001, 255], BF16), (8, [17000001, 8000003], F32)):
+        b, _ = make(hip_ops, sizes, g=g, copy=BF16, bits=bits, seed=12)
+        step_close(b, 3)
+        norm = torch.zeros(1, device="cuda")
+        step_close(b, 4, max_norm=0.5, norm=norm)
+        del b
+
+
+@pytest.mark.parametrize("bits", [32, 8])
 def test_far_magnitudes(bits, hip_ops):
     """Gradients whose squares leave fp32's range below: the norm is summed in 64 bits, second moments that underflow count as zero."""
     b, _ = make(hip_ops, [600], bits=bits, zero=True, spread=False)

@@ -75,12 +75,12 @@ def test_c_entries_refuse():
     p = 1 << 20      # (never read: every call is refused)
     ok = dict(x=p, ldx=8, gamma=0, beta=0, eps=1e-3, z=2 * p, ldz=8, mr=0, P=4, C=8, type=0, ptype=0, stream=0)
     for change in (dict(type=3), dict(type=-1), dict(ptype=1), dict(type=1, ptype=2), dict(P=-1), dict(C=0), dict(C=(1 << 24) + 1), dict(x=0), dict(z=0),
-                   dict(ldz=7), dict(ldx=-1)):
+                   dict(ldz=7), dict(ldx=-1), dict(x=p + 2), dict(type=1, z=2 * p + 1), dict(gamma=p + 1), dict(mr=p + 2), dict(eps=-1.0), dict(eps=float("nan"))):
         assert lib.wdg_layernorm_fwd(*{**ok, **change}.values()) == -1, change
         assert lib.wdg_last_error()
     assert lib.wdg_layernorm_fwd(*{**ok, "P": 0, "x": 0, "z": 0}.values()) == 0
     b = dict(dz=p, lddz=8, x=p, ldx=8, mr=p, gamma=0, dx=2 * p, lddx=8, dg=p, db=p, acc=0, P=4, C=8, type=0, ptype=0, ws=p, wsb=1 << 16, stream=0)
-    for change in (dict(type=5), dict(ptype=2), dict(P=-2), dict(C=0), dict(dz=0), dict(mr=0), dict(dx=0), dict(lddx=5)):
+    for change in (dict(type=5), dict(ptype=2), dict(P=-2), dict(C=0), dict(dz=0), dict(mr=0), dict(dx=0), dict(lddx=5), dict(dg=p + 2), dict(ws=p + 1), dict(dz=p + 1), dict(gamma=p + 2)):
         assert lib.wdg_layernorm_bwd(*{**b, **change}.values()) == -1, change
     for change in (dict(ws=0), dict(wsb=4)):
         assert lib.wdg_layernorm_bwd(*{**b, **change}.values()) == -2, change

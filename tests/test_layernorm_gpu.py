@@ -209,6 +209,32 @@ def test_far_rows(hip_ops):
     backward_close(dz, view(buf), mr, None, view(out), dg, db)
 
 
+@pytest.mark.parametrize("P,C,dtype", [(70000, 1024, F32), (9000, 16384, BF16), (2200000, 32, F16), (17000, 4096, F32), (33000, 2048, BF16)])
+def test_streamed_sizes(P, C, dtype, hip_ops):
+    """Tensors that together pass the last-level cache take non-temporal requests."""
+    gen = torch.Generator(device="cuda").manual_seed(9)
+    x, dz = ((torch.randn(P, C, generator=gen, device="cuda") + 0.5).to(dtype) for _ in range(2))
+    gamma, beta = 1 + 0.3 * torch.randn(C, generator=gen, device="cuda"), torch.randn(C, generator=gen, device="cuda")
+    z, dx, mr = torch.empty_like(x), torch.empty_like(x), torch.empty(P, 2, device="cuda")
+    dg, db = torch.empty(C, device="cuda"), torch.empty(C, device="cuda")
+    hip_ops.layernorm_fwd(x, gamma, beta, EPS, z, mr)
+    hip_ops.layernorm_bwd(dz, x, mr, gamma, dx, dg, db, accumulate=False)
+    for a in range(0, P, 1 + P // 8):                # the rows are checked in pieces: their 64-bit copies are large
+        r = slice(a, a + 1 + P // 8)
+        forward_close(x[r], gamma, beta, z[r], mr[r])
+        backward_close(dz[r], x[r], mr[r], gamma, dx[r], None, None)
+    mag = torch.zeros(C, dtype=torch.float64, device="cuda")
+    sums = torch.zeros(2, C, dtype=torch.float64, device="cuda")
+    for a in range(0, P, 1 + P // 8):
+        r = slice(a, a + 1 + P // 8)
+        g, xh = dz[r].double(), (x[r].double() - mr[r, :1].double()) * mr[r, 1:].double()
+        sums += torch.stack([(g * xh).sum(0), g.sum(0)])
+        mag += (g.abs() * (1 + xh.abs() + 0.5 * (x[r].double().abs() + mr[r, :1].double().abs()) * mr[r, 1:].double())).sum(0)
+    # a thread adds P / (workgroups x rows at a time) rows one after another, at most P / 128 of them here, the partial sums add 512 more
+    lim = (P // 128 + 600) * U * mag
+    assert ((dg.double() - sums[0]).abs() <= lim).all() and ((db.double() - sums[1]).abs() <= lim).all()
+
+
 @pytest.mark.parametrize("P,C,dtype", [(5000, 16, F32), (900, 1155, F16), (1500, 4096, BF16), (40, 20000, BF16)])
 def test_same_bits_every_run(P, C, dtype, hip_ops):
     gen = torch.Generator(device="cuda").manual_seed(6)

@@ -614,7 +614,8 @@ static bool ln_stream(int64_t bytes) { return bytes >= 256ll << 20; }
 static bool ln_types_ok(int type, int ptype) {
     return type >= WDG_F32 && type <= WDG_F16 && (ptype == WDG_F32 || ptype == type);
 }
-static const int64_t LN_MAX_C = 1ll << 24;      // (c / C and the sums' fp32 scale stay exact to rounding)
+static bool ln_aligned(const void* p, int type) { return ((uintptr_t)p & (type == WDG_F32 ? 3 : 1)) == 0; }
+static const int64_t LN_MAX_C = 1ll << 24;      // (C itself is exact in fp32)
 
 template <class T>
 struct LnFwd {
@@ -657,6 +658,9 @@ extern "C" int wdg_layernorm_fwd(const void* x, int64_t ldx, const void* gamma, 
     WDG_CHECK_ARG(P >= 0 && C >= 1 && C <= LN_MAX_C, "bad sizes");
     if (P == 0) return WDG_OK;
     WDG_CHECK_ARG(x && z, "null argument");
+    WDG_CHECK_ARG(eps >= 0.f, "eps has to be a number, not negative");
+    WDG_CHECK_ARG(ln_aligned(x, type) && ln_aligned(z, type) && ln_aligned(gamma, param_type) && ln_aligned(beta, param_type) && ln_aligned(mean_rstd, WDG_F32),
+                  "not aligned to its element");
     WDG_CHECK_ARG(ldx >= 0 && (P == 1 || ldz >= C), "output rows overlap");
     hipStream_t st = (hipStream_t)stream;
     if (type == WDG_F32) return ln_fwd_launch<float, 4>(x, ldx, gamma, beta, param_type, eps, z, ldz, mean_rstd, P, C, type, st);
@@ -733,6 +737,8 @@ extern "C" int wdg_layernorm_bwd(const void* dz, int64_t lddz, const void* x, in
     WDG_CHECK_ARG(P >= 0 && C >= 1 && C <= LN_MAX_C, "bad sizes");
     WDG_CHECK_ARG(P == 0 || (dz && x && mean_rstd && dx), "null argument");
     WDG_CHECK_ARG(lddz >= 0 && ldx >= 0 && (P <= 1 || lddx >= C), "gradient rows overlap");
+    WDG_CHECK_ARG(ln_aligned(dz, type) && ln_aligned(x, type) && ln_aligned(dx, type) && ln_aligned(gamma, param_type) && ln_aligned(mean_rstd, WDG_F32) &&
+                      ln_aligned(dgamma, WDG_F32) && ln_aligned(dbeta, WDG_F32) && ln_aligned(ws, WDG_F32), "not aligned to its element");
     if (P > 0 && (dgamma || dbeta) && (!ws || ws_bytes < wdg_layernorm_bwd_ws_bytes(P, C, type))) {
         wdg_set_error("wdg_layernorm_bwd: workspace too small");
         return WDG_ERR_WORKSPACE;

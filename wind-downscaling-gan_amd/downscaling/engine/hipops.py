@@ -201,6 +201,8 @@ class _AdamWBatch:
             raise RuntimeError("make_adamw lays out and copies a table: not while a graph is captured")
         self.ops, self.state_bits = ops, state_bits
         self.entries = [tuple(e) + (None,) * (4 - len(e)) for e in entries]
+        if any(len(e) != 4 or not torch.is_tensor(e[0]) or not torch.is_tensor(e[1]) or isinstance(e[2], torch.Tensor) or e[2] is None for e in self.entries):
+            raise ValueError("entries: (weights, gradient, decay factor[, copy]) each")
         self.offsets, off = [], 0
         for p, g, decay, copy in self.entries:
             ops._on_device(p, g, copy)
@@ -236,15 +238,15 @@ class _AdamWBatch:
         need = int(ops.lib.wdg_adamw_table_bytes(handle))
         self.table = torch.empty(max(need, 16), dtype=torch.uint8, device=ops.device)
         self.home = ops._raw_stream()
-        native.check(ops.lib.wdg_adamw_bind(handle, self.table.data_ptr(), need, self.home), "adamw_bind")
+        ops._call("adamw_bind", ops.lib.wdg_adamw_bind, handle, self.table.data_ptr(), need)
 
-    def _launch_stream(self):
-        """The stream of one call; what the batch owns is kept from reuse while another stream than its own works on it."""
-        stream = self.ops._raw_stream()
-        if stream != self.home and not torch.cuda.is_current_stream_capturing():
+    def _call(self, what, fn, *args):
+        """One call; what the batch owns is kept from reuse while another stream than its own works on it."""
+        ops = self.ops
+        if ops._raw_stream() != self.home and not torch.cuda.is_current_stream_capturing():
             for t in (self.table, *self.state):
-                t.record_stream(torch.cuda.current_stream(self.ops.device))
-        return stream
+                t.record_stream(torch.cuda.current_stream(ops.device))
+        ops._call(what, fn, *args)
 
     def _scratch(self):
         """Scratch of one call alone: the allocator orders its reuse on this stream, and inside a graph capture it belongs to the graph."""
@@ -273,17 +275,16 @@ class _AdamWBatch:
             args.step_dev = t.data_ptr()
         else:
             args.step = t
-        stream = self._launch_stream()
         scratch = self._scratch() if max_norm is not None else None
-        native.check(self.ops.lib.wdg_adamw_step(self.handle, C.byref(args), _ptr(scratch), self.scratch_bytes, stream), "adamw_step")
+        self._call("adamw_step", self.ops.lib.wdg_adamw_step, self.handle, C.byref(args), _ptr(scratch), self.scratch_bytes)
 
     def grad_norm(self, norm, grad_scale=1.0):
         """norm[0] = grad_scale * sqrt(sum of all gradients' squares), on the device."""
         if norm is None:
             raise ValueError("norm: one fp32 value is wanted")
         p = self._norm_ptr(norm)
-        stream, scratch = self._launch_stream(), self._scratch()
-        native.check(self.ops.lib.wdg_adamw_grad_norm(self.handle, grad_scale, p, scratch.data_ptr(), self.scratch_bytes, stream), "adamw_grad_norm")
+        scratch = self._scratch()
+        self._call("adamw_grad_norm", self.ops.lib.wdg_adamw_grad_norm, self.handle, grad_scale, p, scratch.data_ptr(), self.scratch_bytes)
 
     def moments(self, m_out=None, v_out=None):
         """The moments as numbers, in the state's flat layout: into m_out / v_out ([total], one type of fp32, bf16, fp16)."""
@@ -298,9 +299,8 @@ class _AdamWBatch:
             return
         if not outs:
             return
-        native.check(self.ops.lib.wdg_adamw_moments(self.m.data_ptr(), self.m_scale.data_ptr(), self.v.data_ptr(), self.v_scale.data_ptr(),
-                                                    self.total // self.BLOCK, _ptr(m_out), _ptr(v_out), self.ops.TYPES[outs[0].dtype],
-                                                    self._launch_stream()), "adamw_moments")
+        self._call("adamw_moments", self.ops.lib.wdg_adamw_moments, self.m.data_ptr(), self.m_scale.data_ptr(), self.v.data_ptr(), self.v_scale.data_ptr(),
+                   self.total // self.BLOCK, _ptr(m_out), _ptr(v_out), self.ops.TYPES[outs[0].dtype])
 
     def __del__(self):
         try:
@@ -1137,12 +1137,18 @@ class HipOps:
                 raise ValueError(f"tensor on {t.device}, this backend runs on {self.device}")
 
     def _raw_stream(self):
-        """The current stream of this backend's device as the C ABI takes it, and that device made current: a call costs about as much host
-        time as its launch, and the stream object of the `stream` property alone is a quarter of that."""
-        index = self.device.index
-        if torch.cuda.current_device() != index:
-            torch.cuda.set_device(index)
-        return torch._C._cuda_getCurrentRawStream(index)
+        """The current stream of this backend's device as the C ABI takes it (the stream object of the `stream` property costs a quarter of
+        a small launch)."""
+        return torch._C._cuda_getCurrentRawStream(self.device.index)
+
+    def _call(self, what, fn, *args):
+        """fn(*args, stream) with this backend's device current, as the caller left it afterwards; raises on a status other than 0."""
+        if torch.cuda.current_device() == self.device.index:
+            rc = fn(*args, self._raw_stream())
+        else:
+            with torch.cuda.device(self.device):
+                rc = fn(*args, self._raw_stream())
+        native.check(rc, what)
 
     def _ln_rows(self, name, t, like, out=False):
         """(address, row stride, end of the last row) of a [P, C] tensor of layernorm_fwd / _bwd; `out`: rows are written, so they may not overlap."""
@@ -1203,8 +1209,8 @@ class HipOps:
         self._ln_apart("z", zr, {"x": xr, "gamma": ga, "beta": be, "mean_rstd": mr}, Cn, size)
         if mr[0]:
             self._ln_apart("mean_rstd", mr, {"x": xr, "gamma": ga, "beta": be}, Cn, size)
-        native.check(self.lib.wdg_layernorm_fwd(xr[0], xr[1], ga[0], be[0], eps, zr[0], zr[1], mr[0], P, Cn, self.TYPES[x.dtype],
-                                                self.TYPES[par.dtype] if par is not None else 0, self._raw_stream()), "layernorm_fwd")
+        self._call("layernorm_fwd", self.lib.wdg_layernorm_fwd, xr[0], xr[1], ga[0], be[0], eps, zr[0], zr[1], mr[0], P, Cn, self.TYPES[x.dtype],
+                   self.TYPES[par.dtype] if par is not None else 0)
 
     def layernorm_bwd(self, dz, x, mean_rstd, gamma, dx, dgamma=None, dbeta=None, accumulate=True):
         """Gradients of layernorm_fwd: dx (may be dz or x), and dgamma / dbeta (fp32 [C], added to unless accumulate is False;
@@ -1227,8 +1233,8 @@ class HipOps:
             need = self.lib.wdg_layernorm_bwd_ws_bytes(P, Cn, kind)
             ws = torch.empty(need, dtype=torch.uint8, device=self.device)
             wp = ws.data_ptr()
-        native.check(self.lib.wdg_layernorm_bwd(gr[0], gr[1], xr[0], xr[1], mr[0], ga[0], dr[0], dr[1], dg[0], db[0], bool(accumulate), P, Cn,
-                                                kind, self.TYPES[gamma.dtype] if gamma is not None else 0, wp, need, self._raw_stream()), "layernorm_bwd")
+        self._call("layernorm_bwd", self.lib.wdg_layernorm_bwd, gr[0], gr[1], xr[0], xr[1], mr[0], ga[0], dr[0], dr[1], dg[0], db[0], bool(accumulate),
+                   P, Cn, kind, self.TYPES[gamma.dtype] if gamma is not None else 0, wp, need)
 
     # ---- ConvLSTM cell ----------------------------------------------------------------------
     def lstm_fwd(self, gates, c_prev, c, h, F):
