@@ -398,7 +398,8 @@ int wdg_ln_bwd(const float* dz, int lddz, const float* y, int ldy, const float* 
 
 /* LayerNormalization over the last axis of [P][C] rows of any width (1 <= C <= 2^24) in fp32, bf16 or fp16 (wdg_type), forward and
  * backward (csrc/layernorm.hip) — for the tensors that wdg_ln_fwd / wdg_ln_bwd refuse (16-bit types, C % 4 != 0, C > 1024, odd row
- * strides), with parameter gradients summed in a fixed order: the same bits on every run.
+ * strides), with parameter gradients summed in a fixed order (which depends on the sizes, and on whether dx is written over x or dz): the same
+ * bits on every run.
  *   - x, z, dz, dx: unit channel stride, row strides in elements, aligned to their element only; input rows may coincide
  *     (stride 0 = broadcast); z may be x, and dx may be dz or x, element for element; no other overlap;
  *   - gamma, beta: [C], fp32 or the activations' type (param_type); NULL = ones / zeros;

@@ -130,7 +130,8 @@ def test_in_place_and_broadcast(P, C, dtype, hip_ops):
         a, b = dz.clone(), x.clone()
         g2, b2 = torch.zeros(C, device="cuda"), torch.zeros(C, device="cuda")
         hip_ops.layernorm_bwd(a, b, mr, gamma, a if alias == "dz" else b, g2, b2)
-        assert torch.equal(a if alias == "dz" else b, dx) and torch.equal(g2, dg) and torch.equal(b2, db)
+        assert torch.equal(a if alias == "dz" else b, dx)
+        backward_close(dz, x, mr, gamma, dx, g2, b2)      # (few rows: another order of the sums where dx is a tensor of its own)
     wide = x[:1].expand(P, C)
     hip_ops.layernorm_fwd(wide, gamma, beta, EPS, z, mr)
     forward_close(wide, gamma, beta, z, mr)

@@ -156,7 +156,7 @@ __global__ void __launch_bounds__(NT) wdg_layernorm_fwd_kernel(const T* x, int64
                 for (int j = 0; j < V; ++j) {
                     const float d = TAIL && j < at.dup[k] ? 0.f : (float)xv[u][k].e[j] - s[u];
                     d2[2 * u] += d;
-                    d2[2 * u + 1] += d * d;
+                    d2[2 * u + 1] = fmaf(d, d, d2[2 * u + 1]);
                 }
         }
         wdg_ln_row_sums<L, 2 * U>(d2, red + (L ? 0 : U * 16));
@@ -164,7 +164,7 @@ __global__ void __launch_bounds__(NT) wdg_layernorm_fwd_kernel(const T* x, int64
         for (int u = 0; u < U; ++u) {
             const int64_t p = p0 + u * RG + g;
             const float corr = d2[2 * u] * invC;
-            float var = d2[2 * u + 1] * invC - corr * corr;
+            float var = fmaf(-corr, corr, d2[2 * u + 1] * invC);
             var = var < 0.f ? 0.f : var;                 // (a NaN stays one)
             const float rstd = 1.f / sqrtf(var + eps), shift = -corr * rstd;
             if (p < P) {
@@ -185,10 +185,27 @@ __global__ void __launch_bounds__(NT) wdg_layernorm_fwd_kernel(const T* x, int64
 }
 
 // part: NULL, or one row [dgamma | dbeta] (each of C rounded up to 4) of partial sums per workgroup
+template <class T>
+struct WdgLnBwd {
+    const T* dz;
+    int64_t lddz;
+    const T* x;
+    int64_t ldx;
+    const float* mean_rstd;
+    const void* gamma;
+    int ptype;
+    T* dx;
+    int64_t lddx, P;
+    int C;
+};
+// the rows of workgroup `blk` of `nblk`
 template <class T, int V, int K, int L, int NT, int U, bool TAIL, bool STREAM>
-__global__ void __launch_bounds__(NT) wdg_layernorm_bwd_kernel(const T* dz, int64_t lddz, const T* x, int64_t ldx,
-                                                               const float* __restrict__ mean_rstd, const void* __restrict__ gamma, int ptype,
-                                                               T* dx, int64_t lddx, float* part, int64_t P, int C) {
+__device__ __forceinline__ void wdg_ln_bwd_rows(const WdgLnBwd<T>& q, float* part, int blk, int nblk) {
+    const T *dz = q.dz, *x = q.x;
+    T* dx = q.dx;
+    const float* __restrict__ mean_rstd = q.mean_rstd;
+    const int64_t lddz = q.lddz, ldx = q.ldx, lddx = q.lddx, P = q.P;
+    const int C = q.C;
     constexpr int RG = L ? NT / (L ? L : 1) : 1, COPIES = L ? NT / 64 : 1;      // waves that hold sums of the same columns
     constexpr bool AHEAD = K * U <= 2 && NT <= 512;
     __shared__ float red[L ? 1 : 2 * 2 * U * 16];
@@ -199,12 +216,12 @@ __global__ void __launch_bounds__(NT) wdg_layernorm_bwd_kernel(const T* dz, int6
     float gm[K][V], sg[K][V], sb[K][V];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-        wdg_ln_params<T, V>(gm[k], gamma, ptype, at.col[k], 1.f);
+        wdg_ln_params<T, V>(gm[k], q.gamma, q.ptype, at.col[k], 1.f);
 #pragma unroll
         for (int j = 0; j < V; ++j) sg[k][j] = sb[k][j] = 0.f;
     }
     int turn = 0;
-    const int64_t stride = (int64_t)gridDim.x * (RG * U);
+    const int64_t stride = (int64_t)nblk * (RG * U);
     WdgVec<T, V> x_a[U][K], g_a[U][K];                   // the next rows, on their way while these are worked on (behind the last: again the last)
     float mean_a[U], rstd_a[U];
     auto fetch = [&](int64_t p0) {
@@ -220,8 +237,8 @@ __global__ void __launch_bounds__(NT) wdg_layernorm_bwd_kernel(const T* dz, int6
             }
         }
     };
-    if constexpr (AHEAD) fetch((int64_t)blockIdx.x * (RG * U));
-    for (int64_t p0 = (int64_t)blockIdx.x * (RG * U); p0 < P; p0 += stride) {
+    if constexpr (AHEAD) fetch((int64_t)blk * (RG * U));
+    for (int64_t p0 = (int64_t)blk * (RG * U); p0 < P; p0 += stride) {
         WdgVec<T, V> xv[U][K], gv[U][K];
         float mean[U], rstd[U], s[2 * U];
         if constexpr (!AHEAD) fetch(p0);
@@ -244,11 +261,13 @@ __global__ void __launch_bounds__(NT) wdg_layernorm_bwd_kernel(const T* dz, int6
             for (int k = 0; k < K; ++k)
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
+                    // (every multiply-add is written as one: the instances then give the same bits)
                     const float gg = (float)gv[u][k].e[j], xh = ((float)xv[u][k].e[j] - mean[u]) * rstd[u], a = gg * gm[k][j];
-                    s[2 * u] += TAIL && j < at.dup[k] ? 0.f : a;
-                    s[2 * u + 1] += TAIL && j < at.dup[k] ? 0.f : a * xh;
+                    const float n0 = fmaf(gg, gm[k][j], s[2 * u]), n1 = fmaf(a, xh, s[2 * u + 1]);
+                    s[2 * u] = TAIL && j < at.dup[k] ? s[2 * u] : n0;
+                    s[2 * u + 1] = TAIL && j < at.dup[k] ? s[2 * u + 1] : n1;
                     if (on) {                            // (elements j < dup gather too, and are left out below)
-                        sg[k][j] += gg * xh;
+                        sg[k][j] = fmaf(gg, xh, sg[k][j]);
                         sb[k][j] += gg;
                     }
                 }
@@ -266,7 +285,7 @@ __global__ void __launch_bounds__(NT) wdg_layernorm_bwd_kernel(const T* dz, int6
 #pragma unroll
                     for (int j = 0; j < V; ++j) {
                         const float xh = ((float)xv[u][k].e[j] - mean[u]) * rstd[u];
-                        r.e[j] = (T)(rstd[u] * ((float)gv[u][k].e[j] * gm[k][j] - m1 - xh * m2));
+                        r.e[j] = (T)(rstd[u] * fmaf(-xh, m2, fmaf((float)gv[u][k].e[j], gm[k][j], -m1)));
                     }
                     if (!TAIL || at.dup[k] < V) wdg_vec_store<T, V, STREAM>(dx + p * lddx + at.col[k], r);
                 }
@@ -276,7 +295,7 @@ __global__ void __launch_bounds__(NT) wdg_layernorm_bwd_kernel(const T* dz, int6
     if (!part) return;
     // the workgroup's sums of each column, in a fixed order: lanes of a wave that hold the same columns, then the holders through LDS
     const int Cp = (C + 3) & ~3;
-    float* row = part + (int64_t)blockIdx.x * 2 * Cp;
+    float* row = part + (int64_t)blk * 2 * Cp;
 #pragma unroll
     for (int k = 0; k < K; ++k)
 #pragma unroll
@@ -315,6 +334,46 @@ __global__ void __launch_bounds__(NT) wdg_layernorm_bwd_kernel(const T* dz, int6
                 }
             }
         }
+}
+
+template <class T, int V, int K, int L, int NT, int U, bool TAIL, bool STREAM>
+__global__ void __launch_bounds__(NT) wdg_layernorm_bwd_kernel(const WdgLnBwd<T> q, float* part) {
+    wdg_ln_bwd_rows<T, V, K, L, NT, U, TAIL, STREAM>(q, part, blockIdx.x, gridDim.x);
+}
+
+// Few rows, dx apart from x and dz: both parameter gradients in the same launch, by workgroups of their own behind the `rowblocks` that
+// form dx.  Each owns LN_FEW_COLS columns and reads them of all rows again — from the cache, there are few —, blockDim / LN_FEW_COLS rows
+// at a time, added in that order and then over the threads as a tree.  No partial sums, no second launch (us with / without: 1 x 1024
+// fp32 2.5 / 6.2, 197 x 1155 fp16 4.5 / 8.0, 256 x 16384 bf16 14 / 21).
+constexpr int LN_FEW_ROWS = 256, LN_FEW_COLS = 32;
+template <class T, int V, int K, int L, int NT, int U>
+__global__ void __launch_bounds__(NT) wdg_layernorm_bwd_few_kernel(const WdgLnBwd<T> q, int rowblocks, float* dgamma, float* dbeta, int accumulate) {
+    if ((int)blockIdx.x < rowblocks) {
+        wdg_ln_bwd_rows<T, V, K, L, NT, U, true, false>(q, nullptr, blockIdx.x, rowblocks);
+        return;
+    }
+    __shared__ float sums[2][NT];
+    const int t = threadIdx.x, sets = blockDim.x / LN_FEW_COLS;
+    const int c = ((int)blockIdx.x - rowblocks) * LN_FEW_COLS + t % LN_FEW_COLS;
+    float sg = 0.f, sb = 0.f;
+    if (c < q.C) {
+#pragma unroll 8
+        for (int64_t p = t / LN_FEW_COLS; p < q.P; p += sets) {
+            const float g = (float)q.dz[p * q.lddz + c];
+            sg += g * (((float)q.x[p * q.ldx + c] - q.mean_rstd[2 * p]) * q.mean_rstd[2 * p + 1]);
+            sb += g;
+        }
+    }
+    sums[0][t] = sg;
+    sums[1][t] = sb;
+    __syncthreads();
+    if (t < 2 * LN_FEW_COLS) {
+        const int which = t / LN_FEW_COLS, col = t % LN_FEW_COLS, cc = ((int)blockIdx.x - rowblocks) * LN_FEW_COLS + col;
+        float s = 0.f;
+        for (int w = 0; w < sets; ++w) s += sums[which][w * LN_FEW_COLS + col];
+        float* dst = which ? dbeta : dgamma;
+        if (dst && cc < q.C) dst[cc] = (accumulate ? dst[cc] : 0.f) + s;
+    }
 }
 
 // ---- any width: one block per row, the row read once per pass -------------------------------------------------------------------
@@ -687,28 +746,32 @@ static int ln_finish(const float* part, int rows, int64_t C, float* dgamma, floa
 template <class T>
 struct LnBwd {
     static constexpr int BLOCK_U16 = 1;
-    const T* dz;
-    int64_t lddz;
-    const T* x;
-    int64_t ldx;
-    const float* mean_rstd;
-    const void* gamma;
-    int ptype;
-    T* dx;
-    int64_t lddx;
-    float* part;
-    int64_t P, C;
+    WdgLnBwd<T> q;
+    float *part, *dgamma, *dbeta;
+    int accumulate;
+    bool few;                                            // wdg_layernorm_bwd_few_kernel
     hipStream_t st;
     LnGeom g;
     template <int V, int K, int L, int NT, int U>
     void run() {
-        const bool whole = C == (int64_t)V * K * (L ? L : g.NT);
+        if (few) {
+            const int colblocks = (q.C + LN_FEW_COLS - 1) / LN_FEW_COLS;
+            hipLaunchKernelGGL((wdg_layernorm_bwd_few_kernel<T, V, K, L, NT, U>), dim3(g.blocks + colblocks), dim3(g.NT), 0, st, q, g.blocks, dgamma, dbeta, accumulate);
+            return;
+        }
+        const bool whole = q.C == (int64_t)V * K * (L ? L : g.NT);
         const auto kernel = !whole ? wdg_layernorm_bwd_kernel<T, V, K, L, NT, U, true, false>
-                            : ln_stream(3 * P * C * sizeof(T)) ? wdg_layernorm_bwd_kernel<T, V, K, L, NT, U, false, true>
-                                                                : wdg_layernorm_bwd_kernel<T, V, K, L, NT, U, false, false>;
-        hipLaunchKernelGGL(kernel, dim3(g.blocks), dim3(g.NT), 0, st, dz, lddz, x, ldx, mean_rstd, gamma, ptype, dx, lddx, part, P, (int)C);
+                            : ln_stream(3 * q.P * q.C * sizeof(T)) ? wdg_layernorm_bwd_kernel<T, V, K, L, NT, U, false, true>
+                                                                    : wdg_layernorm_bwd_kernel<T, V, K, L, NT, U, false, false>;
+        hipLaunchKernelGGL(kernel, dim3(g.blocks), dim3(g.NT), 0, st, q, part);
     }
 };
+
+// whether the memory that the rows of two [P][C] tensors of `size` bytes per element span meets
+static bool ln_meet(const void* a, int64_t lda, const void* b, int64_t ldb, int64_t P, int64_t C, int size) {
+    const uintptr_t a0 = (uintptr_t)a, b0 = (uintptr_t)b;
+    return a0 < b0 + (uintptr_t)(((P - 1) * ldb + C) * size) && b0 < a0 + (uintptr_t)(((P - 1) * lda + C) * size);
+}
 
 template <class T, int V>
 static int ln_bwd_launch(const void* dz, int64_t lddz, const void* x, int64_t ldx, const float* mean_rstd, const void* gamma, int ptype,
@@ -716,7 +779,9 @@ static int ln_bwd_launch(const void* dz, int64_t lddz, const void* x, int64_t ld
                          hipStream_t st) {
     const bool params = dgamma || dbeta;
     if (P == 0) return params ? ln_finish(part, 0, C, dgamma, dbeta, accumulate, st) : WDG_OK;
-    LnBwd<T> f = {(const T*)dz, lddz, (const T*)x, ldx, mean_rstd, gamma, ptype, (T*)dx, lddx, params ? part : nullptr, P, C, st, ln_geom(P, C, type, true)};
+    const bool few = params && P <= LN_FEW_ROWS && C <= LN_MAX_ROW && !ln_meet(dx, lddx, x, ldx, P, C, sizeof(T)) && !ln_meet(dx, lddx, dz, lddz, P, C, sizeof(T));
+    LnBwd<T> f = {{(const T*)dz, lddz, (const T*)x, ldx, mean_rstd, gamma, ptype, (T*)dx, lddx, P, (int)C}, params ? part : nullptr, dgamma, dbeta, accumulate,
+                  few, st, ln_geom(P, C, type, true)};
     if (!ln_dispatch<V>(f.g, f)) {
         if (params) {
             hipLaunchKernelGGL((wdg_layernorm_colsum_kernel<T, V>), dim3((unsigned)((C + 256 * V - 1) / (256 * V)), f.g.blocks), dim3(256), 0, st,
@@ -727,7 +792,7 @@ static int ln_bwd_launch(const void* dz, int64_t lddz, const void* x, int64_t ld
                            lddz, (const T*)x, ldx, mean_rstd, gamma, ptype, (T*)dx, lddx, P, C);
     }
     WDG_LAUNCH_CHECK();
-    return params ? ln_finish(part, f.g.blocks, C, dgamma, dbeta, accumulate, st) : WDG_OK;
+    return params && !few ? ln_finish(part, f.g.blocks, C, dgamma, dbeta, accumulate, st) : WDG_OK;
 }
 
 extern "C" int wdg_layernorm_bwd(const void* dz, int64_t lddz, const void* x, int64_t ldx, const float* mean_rstd, const void* gamma,
