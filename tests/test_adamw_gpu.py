@@ -15,7 +15,7 @@ pytestmark = pytest.mark.gpu
 U = 2.0 ** -24
 F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
 HYPER = dict(lr=2e-3, beta1=0.9, beta2=0.99, eps=1e-6, weight_decay=0.1)
-SIZES = {"one": [1], "around a block": [3, 255, 256, 257, 513], "around a chunk": [4095, 4096, 4097, 12288, 1], "with empty ones": [0, 5, 0, 700, 0], "ragged": [70001, 33, 2, 9000]}
+SIZES = {"one": [1], "nine small ones": [300] * 9, "around a block": [3, 255, 256, 257, 513], "around a chunk": [4095, 4096, 4097, 12288, 1], "with empty ones": [0, 5, 0, 700, 0], "ragged": [70001, 33, 2, 9000]}
 
 
 def make(ops, sizes, p=F32, g=F32, copy=None, bits=32, seed=0, shift=0, spread=True, zero=False):

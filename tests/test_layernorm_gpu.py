@@ -11,7 +11,7 @@ pytestmark = pytest.mark.gpu
 U = 2.0 ** -24
 EPS = 1e-3
 F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
-SHAPES = [(1, 1), (5, 2), (3, 7), (9, 8), (2, 9), (130, 16), (33, 100), (64, 64), (700, 33), (3, 255), (4, 1024), (197, 1155), (5, 2048), (6, 4096),
+SHAPES = [(1, 1), (5, 2), (3, 7), (9, 8), (2, 9), (130, 16), (33, 100), (64, 64), (511, 40), (512, 2051), (700, 33), (3, 255), (4, 1024), (197, 1155), (5, 2048), (6, 4096),
           (1, 4097), (37, 5003), (2, 8192), (3, 16384), (2, 16385), (1, 70001)]
 
 

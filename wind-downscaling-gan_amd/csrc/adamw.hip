@@ -14,6 +14,7 @@
 constexpr int AW_CHUNK = 4096;     // elements per record; AW_SMALL of them in short lists (aw_chunk_size)
 constexpr int AW_SMALL = 1024;
 constexpr int AW_BLOCK = 256;      // elements that share a scale of the 8-bit states
+constexpr int AW_ALONE = 8;        // most chunks of a list whose step forms its norm in one launch
 constexpr int AW_PARTS = 256;      // partial sums of the gradient norm: one for each thread of the step's workgroups
 
 struct WdgAdamwChunk {
@@ -45,8 +46,9 @@ struct WdgAdamwHyper {
     double log_b1, log_b2;                        // ... otherwise they come from t in device memory
     const long long* step_dev;
     double grad_scale, max_norm;
-    const double* parts;                          // partial sums of g^2, or NULL: no clipping
+    const double* parts;                          // partial sums of g^2, or NULL
     int nparts;
+    int alone;                                    // > 0: so few chunks that every workgroup adds up the gradients of all of them itself
     float* norm;
 };
 
@@ -129,11 +131,30 @@ __device__ __forceinline__ float wdg_aw_scale(unsigned bits, float& inv) {
     return s;
 }
 
+// a chunk's share of the sum of g^2, per thread of 256; fp64, since a square leaves fp32's range where the gradient itself does not
+template <int CHUNK, bool STREAM, class GT>
+__device__ __forceinline__ double wdg_aw_sumsq(const GT* g, int n) {
+    const int t = (int)(threadIdx.x & 255) * 4;
+    f32x4 v[CHUNK / 1024];
+    if (n == CHUNK) {
+#pragma unroll
+        for (int i = 0; i < CHUNK / 1024; ++i) v[i] = wdg_aw_load<STREAM>(g + i * 1024 + t, 4);
+    } else {
+#pragma unroll
+        for (int i = 0; i < CHUNK / 1024; ++i) v[i] = wdg_aw_load<STREAM>(g + i * 1024 + t, n - i * 1024 - t);
+    }
+    double s = 0.0;
+#pragma unroll
+    for (int i = 0; i < CHUNK / 1024; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s += (double)v[i][j] * (double)v[i][j];
+    return s;
+}
 // clipping: the gradients' factor grad_scale c, the same bits in every workgroup (all add the same numbers in the same order); false
 // where the norm is not finite.  All threads of the workgroup call it once.  `part`: this thread's partial sum, asked for at the start.
 __device__ __forceinline__ bool wdg_aw_clip(const WdgAdamwHyper& h, double part, double* red, float& gs) {
     gs = (float)h.grad_scale;
-    if (!h.parts) return true;
+    if (!h.parts && !h.alone) return true;
     const double s = wdg_aw_wave_sum(part);
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
     __syncthreads();
@@ -254,8 +275,16 @@ __device__ __forceinline__ void wdg_aw_by_grad(const WdgAdamwChunk& q, const Wdg
 template <int BITS, int CHUNK, bool STREAM>
 __global__ void __launch_bounds__(256) wdg_adamw_kernel(const WdgAdamwChunk* __restrict__ table, const WdgAdamwHyper h) {
     __shared__ double red[4];
-    const double part = h.parts && (int)threadIdx.x < h.nparts ? h.parts[threadIdx.x] : 0.0;
+    double part = h.parts && (int)threadIdx.x < h.nparts ? h.parts[threadIdx.x] : 0.0;
     const WdgAdamwChunk q = table[blockIdx.x];
+    if constexpr (CHUNK == AW_SMALL) {
+        for (int c = 0; c < h.alone; ++c) {
+            const WdgAdamwChunk& o = table[c];
+            if (o.g_type == WDG_F32) part += wdg_aw_sumsq<CHUNK, false>(static_cast<const float*>(o.g), o.n);
+            else if (o.g_type == WDG_BF16) part += wdg_aw_sumsq<CHUNK, false>(static_cast<const __bf16*>(o.g), o.n);
+            else part += wdg_aw_sumsq<CHUNK, false>(static_cast<const _Float16*>(o.g), o.n);
+        }
+    }
     float lr_bc1 = h.lr_bc1, rbc2 = h.rbc2;
     if (h.step_dev) {
         // 1 - beta^t = -expm1(t log beta): the difference keeps its digits when beta^t is close to 1
@@ -268,27 +297,9 @@ __global__ void __launch_bounds__(256) wdg_adamw_kernel(const WdgAdamwChunk* __r
     else wdg_aw_by_grad<BITS, CHUNK, STREAM, _Float16>(q, h, part, red, lr_bc1, rbc2);
 }
 
-// ---- sum of g^2 over all chunks; fp64, since a square leaves fp32's range where the gradient itself does not -------------------------
+// ---- sum of g^2 over all chunks ------------------------------------------------------------------------------------------------------
 // Four chunks at a time per workgroup (256 threads each), as many workgroups as the chip holds: the launch reads one tensor, and what it
 // needs is requests in flight.
-template <int CHUNK, bool STREAM, class GT>
-__device__ __forceinline__ double wdg_aw_sumsq(const GT* g, int n) {
-    const int t = (int)(threadIdx.x & 255) * 4;
-    f32x4 v[CHUNK / 1024];
-    if (n == CHUNK) {
-#pragma unroll
-        for (int i = 0; i < CHUNK / 1024; ++i) v[i] = wdg_aw_load<STREAM>(g + i * 1024 + t, 4);
-    } else {
-#pragma unroll
-        for (int i = 0; i < CHUNK / 1024; ++i) v[i] = wdg_aw_load<STREAM>(g + i * 1024 + t, n - i * 1024 - t);
-    }
-    double s = 0.0;
-#pragma unroll
-    for (int i = 0; i < CHUNK / 1024; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) s += (double)v[i][j] * (double)v[i][j];
-    return s;
-}
 template <int CHUNK, bool STREAM>
 __global__ void __launch_bounds__(1024) wdg_adamw_sumsq_kernel(const WdgAdamwChunk* __restrict__ table, int chunks, double* parts) {
     constexpr int R = AW_CHUNK / CHUNK;                   // records at a time
@@ -552,7 +563,10 @@ extern "C" int wdg_adamw_step(const wdg_adamw_batch* b, const wdg_adamw_args* a,
         return WDG_ERR_WORKSPACE;
     }
     if (b->chunks.empty()) return clip && a->norm ? aw_norm(b, 0.0, a->norm, (const double*)scratch, st) : WDG_OK;
-    if (clip) {
+    // up to 8 chunks of 1024: one launch instead of two (3000 elements: 4.0 us instead of 5.5 in a graph, 6.8 instead of 9.6 a call; each
+    // chunk more adds 0.3 us to what every workgroup does by itself)
+    const bool alone = b->chunk == AW_SMALL && b->chunks.size() <= AW_ALONE;
+    if (clip && !alone) {
         const int rc = aw_sumsq(b, (double*)scratch, st);
         if (rc != WDG_OK) return rc;
     }
@@ -576,8 +590,9 @@ extern "C" int wdg_adamw_step(const wdg_adamw_batch* b, const wdg_adamw_args* a,
     h.grad_scale = a->grad_scale;
     if (clip) {
         h.max_norm = a->max_norm;
-        h.parts = (const double*)scratch;
-        h.nparts = aw_parts(b);
+        h.parts = alone ? nullptr : (const double*)scratch;
+        h.nparts = alone ? 0 : aw_parts(b);
+        h.alone = alone ? (int)b->chunks.size() : 0;
         h.norm = a->norm;
     }
     const dim3 grid((unsigned)b->chunks.size());

@@ -342,35 +342,33 @@ __global__ void __launch_bounds__(NT) wdg_layernorm_bwd_kernel(const WdgLnBwd<T>
 }
 
 // Few rows, dx apart from x and dz: both parameter gradients in the same launch, by workgroups of their own behind the `rowblocks` that
-// form dx.  Each owns LN_FEW_COLS columns and reads them of all rows again — from the cache, there are few —, blockDim / LN_FEW_COLS rows
-// at a time, added in that order and then over the threads as a tree.  No partial sums, no second launch (us with / without: 1 x 1024
-// fp32 2.5 / 6.2, 197 x 1155 fp16 4.5 / 8.0, 256 x 16384 bf16 14 / 21).
-constexpr int LN_FEW_ROWS = 256, LN_FEW_COLS = 32;
+// form dx.  Each owns `cols` columns and reads them of all rows again — from the cache, there are few —, blockDim / cols rows at a time,
+// added in that order and then over the threads.  No partial sums, no second launch.
+constexpr int LN_FEW_ROWS = 512;
 template <class T, int V, int K, int L, int NT, int U>
-__global__ void __launch_bounds__(NT) wdg_layernorm_bwd_few_kernel(const WdgLnBwd<T> q, int rowblocks, float* dgamma, float* dbeta, int accumulate) {
+__global__ void __launch_bounds__(NT) wdg_layernorm_bwd_few_kernel(const WdgLnBwd<T> q, int rowblocks, int cols, float* dgamma, float* dbeta, int accumulate) {
     if ((int)blockIdx.x < rowblocks) {
         wdg_ln_bwd_rows<T, V, K, L, NT, U, true, false>(q, nullptr, blockIdx.x, rowblocks);
         return;
     }
     __shared__ float sums[2][NT];
-    const int t = threadIdx.x, sets = blockDim.x / LN_FEW_COLS;
-    const int c = ((int)blockIdx.x - rowblocks) * LN_FEW_COLS + t % LN_FEW_COLS;
+    const int t = threadIdx.x, c0 = ((int)blockIdx.x - rowblocks) * cols, c = c0 + t % cols, sets = blockDim.x / cols;
     float sg = 0.f, sb = 0.f;
     if (c < q.C) {
 #pragma unroll 8
-        for (int64_t p = t / LN_FEW_COLS; p < q.P; p += sets) {
-            const float g = (float)q.dz[p * q.lddz + c];
-            sg += g * (((float)q.x[p * q.ldx + c] - q.mean_rstd[2 * p]) * q.mean_rstd[2 * p + 1]);
+        for (int64_t p = t / cols; p < q.P; p += sets) {
+            const float g = (float)q.dz[p * q.lddz + c], xh = ((float)q.x[p * q.ldx + c] - q.mean_rstd[2 * p]) * q.mean_rstd[2 * p + 1];
+            sg = fmaf(g, xh, sg);
             sb += g;
         }
     }
     sums[0][t] = sg;
     sums[1][t] = sb;
     __syncthreads();
-    if (t < 2 * LN_FEW_COLS) {
-        const int which = t / LN_FEW_COLS, col = t % LN_FEW_COLS, cc = ((int)blockIdx.x - rowblocks) * LN_FEW_COLS + col;
+    if (t < 2 * cols) {
+        const int which = t / cols, cc = c0 + t % cols;
         float s = 0.f;
-        for (int w = 0; w < sets; ++w) s += sums[which][w * LN_FEW_COLS + col];
+        for (int w = 0; w < sets; ++w) s += sums[which][w * cols + t % cols];
         float* dst = which ? dbeta : dgamma;
         if (dst && cc < q.C) dst[cc] = (accumulate ? dst[cc] : 0.f) + s;
     }
@@ -755,8 +753,11 @@ struct LnBwd {
     template <int V, int K, int L, int NT, int U>
     void run() {
         if (few) {
-            const int colblocks = (q.C + LN_FEW_COLS - 1) / LN_FEW_COLS;
-            hipLaunchKernelGGL((wdg_layernorm_bwd_few_kernel<T, V, K, L, NT, U>), dim3(g.blocks + colblocks), dim3(g.NT), 0, st, q, g.blocks, dgamma, dbeta, accumulate);
+            // 16 columns per workgroup, more rows at a time, where that still gives few workgroups; us with 16 / 32 columns / in two launches:
+            // 256 x 64 fp32 3.3 / 4.1 / 5.2, 512 x 1024 bf16 4.1 / 5.5 / 7.7, 512 x 4096 bf16 8.5 / 6.3 / 16, 256 x 16384 bf16 20 / 14 / 21;
+            // with 1024 rows: 64 columns fp32 6.3 / 10 / 5.3
+            const int cols = q.C <= 2048 ? 16 : 32, colblocks = (q.C + cols - 1) / cols;
+            hipLaunchKernelGGL((wdg_layernorm_bwd_few_kernel<T, V, K, L, NT, U>), dim3(g.blocks + colblocks), dim3(g.NT), 0, st, q, g.blocks, cols, dgamma, dbeta, accumulate);
             return;
         }
         const bool whole = q.C == (int64_t)V * K * (L ? L : g.NT);
