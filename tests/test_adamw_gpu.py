@@ -375,13 +375,15 @@ def test_past_32_bits(hip_ops):
     assert (b.m[n - 2000:n] == 127).all() and (b.v[n - 2000:n] == 255).all() and (b.m[:1000] == 0).all() and (b.m[n:] == 0).all()
 
 
-def test_train_step_matches_the_oracle(hip_ops):
+def test_train_step_matches_the_oracle():
     """GanEngine.train_step with AdamW (clipped generator, 32-bit states): both networks' weights after one step against the same
     engine on the 64-bit backend, on the same random stream."""
+    from downscaling.engine.hipops import HipOps
     from downscaling.engine.networks import DiscriminatorNet, GeneratorNet
     from downscaling.engine.trainer import AdamW, GanEngine, PhiloxSource
     from oracle.torch_backend import TorchOps
     from tests.helpers import randomize, rel_err, weights64
+    hip_ops = HipOps("cuda:0")      # (one of its own: a train step picks the streams of its backend)
     B, T, S = 2, 1, 32
     g = torch.Generator().manual_seed(0)
     low, high = (torch.randn(B, T, S, S, c, generator=g, dtype=torch.float64) for c in (3, 2))
