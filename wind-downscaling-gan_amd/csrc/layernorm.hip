@@ -12,6 +12,10 @@
 // Numerics: statistics, sums and the normalised value are fp32 whatever the tensors' type; z and dx are rounded once, on store.  The
 // mean is corrected by the mean of (x - mean), which is what fp32 left out of it, so a row with an offset of many standard deviations
 // keeps its digits; the variance is the sum of squares about the corrected mean.
+//
+// Bound: HBM where the tensors are larger than the caches — forward 2, backward 3 times the tensor, which is what the counters show.
+// 16384 x 4096 bf16 forward 48.7 us (5.5 TB/s), backward 76 (5.3, the parameter sums' launch included); 65536 x 1024 fp32 90 and 135 us
+// (5.9 and 6.0 TB/s); 2097152 x 16 fp32 backward 75 us (5.4).  A large copy reaches 5.3 TB/s on the same card.
 #include "vec.h"
 #include <algorithm>
 
@@ -374,7 +378,8 @@ __global__ void __launch_bounds__(NT) wdg_layernorm_bwd_few_kernel(const WdgLnBw
     }
 }
 
-// ---- any width: one block per row, the row read once per pass -------------------------------------------------------------------
+// ---- any width: one block per row, the row read once per pass (from the cache, but for the first) -------------------------------------
+// 4096 x 32768 bf16: forward 181 us (3.0 TB/s of what the passes after the first do not count), backward 326 (2.5).
 // The last, partial vector of a row is taken element by element (never beyond the row: what follows may be another row, or nothing).
 constexpr int LNW_NT = 1024;
 

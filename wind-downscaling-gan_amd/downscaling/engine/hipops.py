@@ -203,14 +203,14 @@ class _AdamWBatch:
         self.entries = [tuple(e) + (None,) * (4 - len(e)) for e in entries]
         if any(len(e) != 4 or not torch.is_tensor(e[0]) or not torch.is_tensor(e[1]) or isinstance(e[2], torch.Tensor) or e[2] is None for e in self.entries):
             raise ValueError("entries: (weights, gradient, decay factor[, copy]) each")
-        self.offsets, off = [], 0
+        self.offsets, off, types, device = [], 0, ops.TYPES, ops.device
         for p, g, decay, copy in self.entries:
-            ops._on_device(p, g, copy)
-            for name, t, dtypes in (("weights", p, ops.TYPES), ("gradient", g, ops.TYPES), ("copy", copy, (torch.bfloat16, torch.float16))):
-                if t is None and name == "copy":
-                    continue
-                if t.dtype not in dtypes or t.shape != p.shape or not t.is_contiguous():
-                    raise ValueError(f"{name}: a contiguous {tuple(p.shape)} tensor of {' or '.join(str(d) for d in dtypes)} is wanted, got {t.dtype} {tuple(t.shape)}")
+            shape = p.shape
+            if not (p.dtype in types and g.dtype in types and g.shape == shape and p.is_contiguous() and g.is_contiguous() and p.device == device
+                    and g.device == device and (copy is None or (copy.dtype in (torch.bfloat16, torch.float16) and copy.shape == shape
+                                                                 and copy.is_contiguous() and copy.device == device))):
+                raise ValueError("weights, gradient and copy: contiguous tensors of one shape on " + str(device) + ", fp32, bf16 or fp16 (a copy bf16 or fp16), got "
+                                 + ", ".join(f"{t.dtype} {tuple(t.shape)} on {t.device}" for t in (p, g, copy) if t is not None))
             self.offsets.append(off)
             off += -(-p.numel() // self.BLOCK) * self.BLOCK
         self.total = off
@@ -226,11 +226,12 @@ class _AdamWBatch:
         self.m_scale, self.v_scale = state[2:] if state_bits == 8 else (None, None)
         self.handle = None
         arr = (native.AdamWTensor * max(len(self.entries), 1))()
-        for i, ((p, g, decay, copy), o) in enumerate(zip(self.entries, self.offsets)):
-            at = lambda t, k: 0 if t is None else t.data_ptr() + k * t.element_size()      # noqa: E731
-            arr[i] = native.AdamWTensor(p.data_ptr(), g.data_ptr(), at(self.m, o), at(self.v, o), at(self.m_scale, o // self.BLOCK),
-                                        at(self.v_scale, o // self.BLOCK), _ptr(copy), p.numel(), ops.TYPES[p.dtype], ops.TYPES[g.dtype],
-                                        0 if copy is None else ops.TYPES[copy.dtype], float(decay))
+        pm, pv, pms, pvs = self.m.data_ptr(), self.v.data_ptr(), _ptr(self.m_scale), _ptr(self.v_scale)
+        each, scale = (4, 0) if state_bits == 32 else (1, 4)          # bytes of a state's element, of a block's scale
+        for a, (p, g, decay, copy), o in zip(arr, self.entries, self.offsets):
+            k = scale * (o // self.BLOCK)
+            a.p, a.g, a.m, a.v, a.m_scale, a.v_scale, a.copy, a.n = p.data_ptr(), g.data_ptr(), pm + each * o, pv + each * o, pms + k, pvs + k, _ptr(copy), p.numel()
+            a.p_type, a.g_type, a.copy_type, a.decay = types[p.dtype], types[g.dtype], 0 if copy is None else types[copy.dtype], decay
         handle = C.c_void_p()
         native.check(ops.lib.wdg_adamw_create(C.byref(handle), arr, len(self.entries), state_bits), "adamw_create")
         self.handle = handle
