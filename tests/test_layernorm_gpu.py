@@ -3,7 +3,8 @@
 Tolerances, derived: u = 2^-24 is half a step of fp32.  A thread adds at most `seq` terms one after another and the rest is a tree of at
 most 16 levels, so a mean over the row is off by at most K u times the mean of the terms' magnitudes, K = seq + 16.  The centred value
 x - mean therefore carries K u (|x - mean| + mean |x - mean|), rstd a relative (K + 8) u, and scaling, shifting and the centred value's own
-rounding a few u of the terms that they add.  Both tensors round once more on store: finfo.eps / 2 of the value."""
+rounding a few u of the terms that they add.  The first mean is off by K u |mean|; the mean of (x - mean) takes that out but for K u of it,
+(K u)^2 |mean| — all there is in a row of equal values.  Both tensors round once more on store: finfo.eps / 2 of the value."""
 import pytest
 import torch
 
@@ -38,7 +39,7 @@ def forward_close(x, gamma, beta, z, mr, what=""):
     ref = d * rstd * g + b
     K = chain(C)
     spread = d.abs().mean(1, keepdim=True)
-    tol = U * ((K * (d.abs() + spread) * rstd + (K + 8) * (d * rstd).abs()) * g.abs() + 4 * (b.abs() + ref.abs())) + torch.finfo(z.dtype).eps / 2 * ref.abs() + 1e-30
+    tol = U * ((K * (d.abs() + spread + K * U * mean.abs()) * rstd + (K + 8) * (d * rstd).abs()) * g.abs() + 4 * (b.abs() + ref.abs())) + torch.finfo(z.dtype).eps / 2 * ref.abs() + 1e-30
     if z.dtype == F16:
         tol = tol + 2.0 ** -25                                                         # half of fp16's smallest step
     assert ((z.double() - ref).abs() <= tol).all(), (what, float(((z.double() - ref).abs() / tol).max()))

@@ -379,7 +379,7 @@ __global__ void __launch_bounds__(NT) wdg_layernorm_bwd_few_kernel(const WdgLnBw
 }
 
 // ---- any width: one block per row, the row read once per pass (from the cache, but for the first) -------------------------------------
-// 4096 x 32768 bf16: forward 181 us (3.0 TB/s of what the passes after the first do not count), backward 326 (2.5).
+// 4096 x 32768 bf16: forward 181 us (3.0 TB/s, each tensor counted once), backward 326 (2.5).
 // The last, partial vector of a row is taken element by element (never beyond the row: what follows may be another row, or nothing).
 constexpr int LNW_NT = 1024;
 
