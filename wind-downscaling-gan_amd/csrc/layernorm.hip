@@ -740,8 +740,12 @@ extern "C" size_t wdg_layernorm_bwd_ws_bytes(int64_t P, int64_t C, int type) {
 
 static int ln_finish(const float* part, int rows, int64_t C, float* dgamma, float* dbeta, int accumulate, hipStream_t st) {
     const int64_t cols = 2 * ((C + 3) & ~3ll);
+    // columns per workgroup by how many workgroups they leave: with 64 / 32, us of the whole backward: 3000 x 1024 bf16 12.1 / 10.8,
+    // 1537 x 5003 fp16 18.4 / 19.5
     if (cols <= 256)
         hipLaunchKernelGGL(wdg_layernorm_finish_kernel<16>, dim3((unsigned)((cols + 15) / 16)), dim3(1024), 0, st, part, rows, C, dgamma, dbeta, accumulate);
+    else if (cols <= 4096)
+        hipLaunchKernelGGL(wdg_layernorm_finish_kernel<32>, dim3((unsigned)((cols + 31) / 32)), dim3(1024), 0, st, part, rows, C, dgamma, dbeta, accumulate);
     else
         hipLaunchKernelGGL(wdg_layernorm_finish_kernel<64>, dim3((unsigned)((cols + 63) / 64)), dim3(1024), 0, st, part, rows, C, dgamma, dbeta, accumulate);
     WDG_LAUNCH_CHECK();
