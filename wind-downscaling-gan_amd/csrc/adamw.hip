@@ -175,7 +175,9 @@ __device__ __forceinline__ bool wdg_aw_clip(const WdgAdamwHyper& h, double part,
 template <int BITS, int CHUNK, bool STREAM, class PT, class GT, bool FULL>
 __device__ __forceinline__ void wdg_aw_chunk(const WdgAdamwChunk& q, const WdgAdamwHyper& h, double part, double* red, float lr_bc1, float rbc2) {
     constexpr int QUADS = CHUNK / 1024, UN = FULL ? QUADS : 1;
-    const float keep = 1.f - h.lr_wd * q.decay;
+    // the decay's factor 1 - lr weight_decay d as two numbers: alone the first is a multiple of 2^-24, and every step of a run would decay by
+    // the same wrong amount (lr weight_decay = 4e-8 by half too much, 2e-8 not at all)
+    const float lwd = h.lr_wd * q.decay, keep = 1.f - lwd, keep_rest = (1.f - keep) - lwd;
     PT* p = static_cast<PT*>(q.p);
     const GT* g = static_cast<const GT*>(q.g);
     const int lane = threadIdx.x & 63;
@@ -224,7 +226,9 @@ __device__ __forceinline__ void wdg_aw_chunk(const WdgAdamwChunk& q, const WdgAd
                 const float a = h.b1 * m[k][j] + h.c1 * gj, b = h.b2 * v[k][j] + h.c2 * (gj * gj);
                 m[k][j] = a;
                 v[k][j] = b;
-                w[k][j] = w[k][j] * keep - lr_bc1 * (a / (sqrtf(b) * rbc2 + h.eps));
+                // (the small product of a finite weight: an infinite one stays infinite)
+                const float rest = fmaf(__builtin_amdgcn_fmed3f(w[k][j], -3.4028235e38f, 3.4028235e38f), keep_rest, -lr_bc1 * (a / (sqrtf(b) * rbc2 + h.eps)));
+                w[k][j] = fmaf(w[k][j], keep, rest);
                 if constexpr (BITS == 8) {               // (from the scalars: a bit cast of a vector's element would take element 0)
                     tm = max(tm, j < n ? __builtin_bit_cast(unsigned, a) & 0x7fffffffu : 0u);
                     tv = max(tv, j < n ? __builtin_bit_cast(unsigned, b) & 0x7fffffffu : 0u);
