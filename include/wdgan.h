@@ -722,9 +722,10 @@ int wdg_adam_tf(float* p, const float* g, float* m, float* v, int64_t n, float l
  * finite leaves weights, copies and states as they were.  Without it a NaN or an infinity goes where the formula takes it.
  *
  * 8-bit states: every 256 consecutive elements of a tensor (the last block may be shorter) share two fp32 scales, M = max |m| and
- * V = max v, and hold   m = M q |q| / 127^2, q = -127 .. 127 (int8),   v = V (q / 255)^4, q = 0 .. 255 (uint8),
- * q rounded to nearest on the companded value and, for v > 0, at least 1: the second moment of an element that has one never reads as
- * zero.  Scales below 2^-126 count as zero.  A block that a value which is not finite reaches is NaN from then on.
+ * V = max(max v, 2^-94) (0 where all v are), and hold   m = M q |q| / 127^2, q = -127 .. 127 (int8),   v = V (q / 255)^4, q = 0 .. 255
+ * (uint8), q rounded to nearest on the companded value and, for v > 0, at least 1: a second moment that fp32 holds above zero is written so
+ * that it reads above zero, as a normal number.  M below 2^-126 counts as zero.  A block that a value which is not finite reaches is NaN
+ * from then on.
  *
  * Tensors: p, g, copy and fp32 states are aligned to their element; 8-bit states to 4 bytes, and their code arrays span whole blocks of
  * 256 bytes (codes behind the last element are written as zero).  n == 0 is allowed.  No written range may meet another one or a

@@ -724,7 +724,7 @@ class TorchOps:
                 x = x.view(-1, 256)
                 top = x.abs().amax(1, keepdim=True)
                 top = torch.where(x.isfinite().all(1, keepdim=True), top, torch.full_like(top, float("nan")))
-                top = torch.where(top < 2.0 ** -126, torch.zeros_like(top), top)
+                top = torch.where((top > 0) & (top < 2.0 ** -94), torch.full_like(top, 2.0 ** -94), top) if second else torch.where(top < 2.0 ** -126, torch.zeros_like(top), top)
                 part = torch.where((top > 0) & x.isfinite(), x.abs() / top, torch.zeros_like(x))
                 if second:
                     q = torch.where(part > 0, torch.round(255 * part ** 0.25).clamp(min=1), part)

@@ -121,12 +121,17 @@ __device__ __forceinline__ double wdg_aw_wave_sum(double v) {
 }
 // A block's scale from the largest bit pattern of its magnitudes (as integers: above infinity come the NaNs, which a float maximum would
 // drop).  inv = 1 / scale, 0 where the block holds zeros alone; a block that is not finite gets a NaN for its scale.
+// First moments below 2^-126 count as zero: the scale's reciprocal would not be a number.  The scale of second moments is 2^-94 at least,
+// so that code 1, a 255^4th of it, is a normal number: what is above zero does not read as zero.
+template <bool SECOND>
 __device__ __forceinline__ float wdg_aw_scale(unsigned bits, float& inv) {
+    constexpr unsigned least = SECOND ? (127u - 94u) << 23 : 1u << 23;
     if (bits >= 0x7f800000u) {
         inv = 0.f;
         return __builtin_nanf("");
     }
-    if (bits < 0x00800000u) {                     // below 2^-126: its reciprocal would not be a number
+    if (SECOND && bits != 0) bits = max(bits, least);
+    if (bits < least) {
         inv = 0.f;
         return 0.f;
     }
@@ -242,15 +247,16 @@ __device__ __forceinline__ void wdg_aw_chunk(const WdgAdamwChunk& q, const WdgAd
                 wdg_aw_store<STREAM>(static_cast<float*>(q.v) + e, n, v[k]);
             } else {
                 float im, iv;
-                const float nm = wdg_aw_scale(wdg_wave_umax(tm), im), nv = wdg_aw_scale(wdg_wave_umax(tv), iv);
+                const float nm = wdg_aw_scale<false>(wdg_wave_umax(tm), im), nv = wdg_aw_scale<true>(wdg_wave_umax(tv), iv);
                 unsigned om = 0, ov = 0;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     if (j >= n) continue;
                     // both companding roots on the hardware square root (one unit in the last place of a value that is rounded to
                     // 1 / 127 or 1 / 255): only a value that close to the border between two codes can take the other one
-                    const float a = rintf(127.f * __builtin_amdgcn_sqrtf(fabsf(m[k][j]) * im)), r = v[k][j] * iv;
-                    const float b = r > 0.f ? fmaxf(rintf(255.f * __builtin_amdgcn_sqrtf(__builtin_amdgcn_sqrtf(r))), 1.f) : 0.f;
+                    const float a = rintf(127.f * __builtin_amdgcn_sqrtf(fabsf(m[k][j]) * im));
+                    // (v itself decides whether there is one: its quotient to the block's largest may be below fp32's range)
+                    const float b = v[k][j] > 0.f ? fmaxf(rintf(255.f * __builtin_amdgcn_sqrtf(__builtin_amdgcn_sqrtf(v[k][j] * iv))), 1.f) : 0.f;
                     const int ai = im > 0.f ? (int)(m[k][j] < 0.f ? -a : a) : 0, bi = iv > 0.f ? (int)b : 0;
                     om |= ((unsigned)ai & 255u) << (8 * j);
                     ov |= ((unsigned)bi & 255u) << (8 * j);
