@@ -729,7 +729,8 @@ int wdg_adam_tf(float* p, const float* g, float* m, float* v, int64_t n, float l
  *
  * Tensors: p, g, copy and fp32 states are aligned to their element; 8-bit states to 4 bytes, and their code arrays span whole blocks of
  * 256 bytes (codes behind the last element are written as zero).  n == 0 is allowed.  No written range may meet another one or a
- * gradient: create refuses.  decay: factor of weight_decay for this tensor (0: not decayed).
+ * gradient: create refuses, and so do the calls for a norm, a step count or scratch inside the list's tensors or each other.  decay:
+ * factor of weight_decay for this tensor (0: not decayed).
  * ------------------------------------------------------------------------------------------ */
 typedef struct wdg_adamw_tensor {
     void* p;                  /* weights, updated in place */

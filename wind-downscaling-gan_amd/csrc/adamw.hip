@@ -13,6 +13,7 @@
 #include <algorithm>
 #include <exception>
 #include <math.h>
+#include <utility>
 #include <vector>
 
 constexpr int AW_CHUNK = 4096;     // elements per record; AW_SMALL of them in short lists (aw_chunk_size)
@@ -34,8 +35,15 @@ struct WdgAdamwChunk {
     float decay;
     int pad2;
 };
+struct AwRange {
+    uintptr_t begin, end;
+    bool written;
+};
+
 struct wdg_adamw_batch {
     std::vector<WdgAdamwChunk> chunks;
+    std::vector<AwRange> ranges;                  // the tensors' memory by address (gradients may share theirs) ...
+    std::vector<uintptr_t> ends;                  // ... and the furthest end up to each of them
     int bits = 32;
     int chunk = AW_CHUNK;
     int64_t bytes = 0, grad_bytes = 0;            // of everything a step touches, of the gradients alone
@@ -412,11 +420,6 @@ static bool aw_stream_step(const wdg_adamw_batch* b) { return b->bytes >= 96ll <
 // 159 without; 128 M (488 MiB) 703 and 792.
 static bool aw_stream_norm(const wdg_adamw_batch* b) { return b->grad_bytes >= 192ll << 20; }
 
-struct AwRange {
-    uintptr_t begin, end;
-    bool written;
-};
-
 static int aw_create(wdg_adamw_batch** out, const wdg_adamw_tensor* tensors, int n, int bits) {
     std::vector<AwRange> ranges;
     int64_t chunks = 0, total = 0, grads = 0;
@@ -466,6 +469,7 @@ static int aw_create(wdg_adamw_batch** out, const wdg_adamw_tensor* tensors, int
     b->grad_bytes = grads;
     try {
         b->chunks.reserve((size_t)(chunks * (AW_CHUNK / b->chunk)));
+        b->ends.reserve(ranges.size());
     } catch (...) {
         delete b;
         throw;
@@ -490,8 +494,31 @@ static int aw_create(wdg_adamw_batch** out, const wdg_adamw_tensor* tensors, int
             b->chunks.push_back(q);
         }
     }
+    for (const AwRange& r : ranges) b->ends.push_back(std::max(b->ends.empty() ? 0 : b->ends.back(), r.end));
+    b->ranges = std::move(ranges);
     *out = b;
     return WDG_OK;
+}
+
+// whether `bytes` at p meet a tensor of the list
+static bool aw_meets(const wdg_adamw_batch* b, const void* p, size_t bytes) {
+    if (!p) return false;
+    const uintptr_t begin = (uintptr_t)p, end = begin + bytes;
+    const auto behind = std::lower_bound(b->ranges.begin(), b->ranges.end(), end, [](const AwRange& r, uintptr_t e) { return r.begin < e; });
+    return behind != b->ranges.begin() && b->ends[behind - b->ranges.begin() - 1] > begin;
+}
+static bool aw_apart(const void* p, size_t np, const void* q, size_t nq) {
+    return !p || !q || (uintptr_t)p + np <= (uintptr_t)q || (uintptr_t)q + nq <= (uintptr_t)p;
+}
+// what a call writes and reads beside the list's tensors has to be memory of its own: NULL, or what is not
+static const char* aw_beside(const wdg_adamw_batch* b, const void* norm, const void* step_dev, const void* scratch) {
+    if (aw_meets(b, norm, sizeof(float))) return "the norm overlaps a tensor of the list";
+    if (aw_meets(b, step_dev, sizeof(int64_t))) return "the step count overlaps a tensor of the list";
+    if (aw_meets(b, scratch, AW_PARTS * sizeof(double))) return "the scratch overlaps a tensor of the list";
+    if (!aw_apart(norm, sizeof(float), scratch, AW_PARTS * sizeof(double)) || !aw_apart(norm, sizeof(float), step_dev, sizeof(int64_t)) ||
+        !aw_apart(step_dev, sizeof(int64_t), scratch, AW_PARTS * sizeof(double)))
+        return "norm, step count and scratch overlap";
+    return nullptr;
 }
 
 extern "C" int wdg_adamw_create(wdg_adamw_batch** out, const wdg_adamw_tensor* tensors, int n, int state_bits) {
@@ -547,12 +574,14 @@ static int aw_norm(const wdg_adamw_batch* b, double scale, float* norm, const do
 extern "C" int wdg_adamw_grad_norm(const wdg_adamw_batch* b, double grad_scale, float* norm, void* scratch, size_t scratch_bytes,
                                    wdg_stream stream) {
     WDG_CHECK_ARG(b && norm, "null argument");
-    WDG_CHECK_ARG(b->chunks.empty() || b->table, "wdg_adamw_bind has not been called");
     WDG_CHECK_ARG(grad_scale >= 0.0 && grad_scale < INFINITY, "gradient scale");
     if (!scratch || !aw_aligned(scratch, 8) || scratch_bytes < wdg_adamw_scratch_bytes()) {
         wdg_set_error("wdg_adamw_grad_norm: scratch too small or not aligned");
         return WDG_ERR_WORKSPACE;
     }
+    const char* beside = aw_beside(b, norm, nullptr, scratch);
+    WDG_CHECK_ARG(!beside, beside);
+    WDG_CHECK_ARG(b->chunks.empty() || b->table, "wdg_adamw_bind has not been called");
     const int rc = aw_sumsq(b, (double*)scratch, (hipStream_t)stream);
     return rc != WDG_OK ? rc : aw_norm(b, grad_scale, norm, (const double*)scratch, (hipStream_t)stream);
 }
@@ -565,7 +594,6 @@ static auto aw_step_kernel(const wdg_adamw_batch* b) {
 
 extern "C" int wdg_adamw_step(const wdg_adamw_batch* b, const wdg_adamw_args* a, void* scratch, size_t scratch_bytes, wdg_stream stream) {
     WDG_CHECK_ARG(b && a, "null argument");
-    WDG_CHECK_ARG(b->chunks.empty() || b->table, "wdg_adamw_bind has not been called");
     WDG_CHECK_ARG(a->beta1 >= 0.0 && a->beta1 < 1.0 && a->beta2 >= 0.0 && a->beta2 < 1.0, "beta1 and beta2 have to be in [0, 1)");
     WDG_CHECK_ARG(a->eps >= 0.0 && a->lr >= 0.0 && a->weight_decay >= 0.0 && a->grad_scale >= 0.0 && a->eps < INFINITY && a->lr < INFINITY &&
                       a->weight_decay < INFINITY && a->grad_scale < INFINITY && a->max_norm < INFINITY, "lr, eps, weight decay and gradient scale: finite, not negative");
@@ -576,6 +604,9 @@ extern "C" int wdg_adamw_step(const wdg_adamw_batch* b, const wdg_adamw_args* a,
         wdg_set_error("wdg_adamw_step: scratch too small or not aligned");
         return WDG_ERR_WORKSPACE;
     }
+    const char* beside = aw_beside(b, clip ? a->norm : nullptr, a->step_dev, clip ? scratch : nullptr);
+    WDG_CHECK_ARG(!beside, beside);
+    WDG_CHECK_ARG(b->chunks.empty() || b->table, "wdg_adamw_bind has not been called");
     if (b->chunks.empty()) return clip && a->norm ? aw_norm(b, 0.0, a->norm, (const double*)scratch, st) : WDG_OK;
     // up to 8 chunks of 1024: one launch instead of two (3000 elements: 4.0 us instead of 5.5 in a graph, 6.8 instead of 9.6 a call; each
     // chunk more adds 0.3 us to what every workgroup does by itself)
