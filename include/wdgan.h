@@ -763,7 +763,8 @@ size_t wdg_adamw_scratch_bytes(void);
 int wdg_adamw_step(const wdg_adamw_batch* b, const wdg_adamw_args* args, void* scratch, size_t scratch_bytes, wdg_stream stream);
 /* norm[0] = grad_scale sqrt(sum g^2) over all gradients of the batch (0 for none). */
 int wdg_adamw_grad_norm(const wdg_adamw_batch* b, double grad_scale, float* norm, void* scratch, size_t scratch_bytes, wdg_stream stream);
-/* The values that 8-bit states stand for: m_out / v_out [blocks * 256] of type out_type (either may be NULL). */
+/* The values that 8-bit states stand for: m_out / v_out [blocks * 256] of type out_type (either may be NULL), apart from each other and
+ * from the states. */
 int wdg_adamw_moments(const void* m, const float* m_scale, const void* v, const float* v_scale, int64_t blocks, void* m_out, void* v_out,
                       int out_type, wdg_stream stream);
 /* Zero 1..16 element ranges [begin, end) of a flat fp32 buffer in one launch (begin_end: host array of n pairs, every value a

@@ -653,6 +653,11 @@ extern "C" int wdg_adamw_moments(const void* m, const float* m_scale, const void
     if (blocks == 0 || (!m_out && !v_out)) return WDG_OK;
     WDG_CHECK_ARG((!m_out || (m && m_scale)) && (!v_out || (v && v_scale)), "null argument");
     WDG_CHECK_ARG(aw_aligned(m, 4) && aw_aligned(v, 4) && aw_aligned(m_out, aw_bytes(out_type)) && aw_aligned(v_out, aw_bytes(out_type)), "alignment");
+    const size_t n = (size_t)blocks * AW_BLOCK, out = n * aw_bytes(out_type), scales = (size_t)blocks * sizeof(float);
+    bool apart = aw_apart(m_out, out, v_out, out);
+    for (const void* o : {m_out, v_out})
+        apart = apart && aw_apart(o, out, m, n) && aw_apart(o, out, v, n) && aw_apart(o, out, m_scale, scales) && aw_apart(o, out, v_scale, scales);
+    WDG_CHECK_ARG(apart, "the moments read out overlap each other or the states");
     const long long sixteens = blocks * (AW_BLOCK / 16);
     const dim3 grid((unsigned)std::min<long long>((sixteens + 255) / 256, 16384), 2);
     hipStream_t st = (hipStream_t)stream;

@@ -288,12 +288,16 @@ class _AdamWBatch:
         self._call("adamw_grad_norm", self.ops.lib.wdg_adamw_grad_norm, self.handle, grad_scale, p, scratch.data_ptr(), self.scratch_bytes)
 
     def moments(self, m_out=None, v_out=None):
-        """The moments as numbers, in the state's flat layout: into m_out / v_out ([total], one type of fp32, bf16, fp16)."""
+        """The moments as numbers, in the state's flat layout: into m_out / v_out ([total], one type of fp32, bf16, fp16), apart from each other
+        and from the states."""
         outs = [t for t in (m_out, v_out) if t is not None]
         self.ops._on_device(*outs)
         if any(t.dtype not in self.ops.TYPES or t.dtype != outs[0].dtype or tuple(t.shape) != (self.total,) or not t.is_contiguous() for t in outs):
             raise ValueError(f"contiguous [{self.total}] tensors of one type of {', '.join(str(d) for d in self.ops.TYPES)} are wanted")
         if self.state_bits == 32:
+            at = lambda t: (0, 0) if t is None else (t.data_ptr(), t.data_ptr() + t.numel() * t.element_size())      # noqa: E731
+            self.ops._ln_apart("m_out", at(m_out), {"v_out": at(v_out), "the second moment": at(self.v)}, 0, 0)
+            self.ops._ln_apart("v_out", at(v_out), {"the first moment": at(self.m)}, 0, 0)
             for t, s in ((m_out, self.m), (v_out, self.v)):
                 if t is not None:
                     t.copy_(s)
