@@ -719,7 +719,8 @@ int wdg_adam_tf(float* p, const float* g, float* m, float* v, int64_t n, float l
  *   m = beta1 m + (1 - beta1) g';  v = beta2 v + (1 - beta2) g'^2
  *   p = p (1 - lr weight_decay decay) - lr / (1 - beta1^t) m / (sqrt(v / (1 - beta2^t)) + eps);  copy = p rounded to its type
  * Arithmetic is fp32 (the norm's sum fp64) whatever the tensors' types; p is rounded once.  With max_norm > 0 a norm that is not
- * finite leaves weights, copies and states as they were.  Without it a NaN or an infinity goes where the formula takes it.
+ * finite, as the fp32 value that goes to args->norm, leaves weights, copies and states as they were.  Without it a NaN or an infinity goes
+ * where the formula takes it.
  *
  * 8-bit states: every 256 consecutive elements of a tensor (the last block may be shorter) share two fp32 scales, M = max |m| and
  * V = max(max v, 2^-94) (0 where all v are), and hold   m = M q |q| / 127^2, q = -127 .. 127 (int8),   v = V (q / 255)^4, q = 0 .. 255

@@ -738,7 +738,7 @@ class TorchOps:
                     self.grad_norm(n, grad_scale)
                     if norm is not None:
                         norm.copy_(n)
-                    if not math.isfinite(float(n)):
+                    if not math.isfinite(float(n.float())):      # (as fp32 hands it out)
                         return
                     c = max_norm / max(float(n), max_norm)
                 ms, vs = self.values()

@@ -168,7 +168,7 @@ __device__ __forceinline__ double wdg_aw_sumsq(const GT* g, int n) {
     return s;
 }
 // clipping: the gradients' factor grad_scale c, the same bits in every workgroup (all add the same numbers in the same order); false
-// where the norm is not finite.  All threads of the workgroup call it once.  `part`: this thread's partial sum, asked for at the start.
+// where the norm is not finite in fp32.  All threads of the workgroup call it once.  `part`: this thread's partial sum, asked for at the start.
 __device__ __forceinline__ bool wdg_aw_clip(const WdgAdamwHyper& h, double part, double* red, float& gs) {
     gs = (float)h.grad_scale;
     if (!h.parts && !h.alone) return true;
@@ -177,7 +177,7 @@ __device__ __forceinline__ bool wdg_aw_clip(const WdgAdamwHyper& h, double part,
     __syncthreads();
     const double norm = h.grad_scale * sqrt((red[0] + red[1]) + (red[2] + red[3]));
     if (h.norm && blockIdx.x == 0 && threadIdx.x == 0) h.norm[0] = (float)norm;
-    if (!(norm <= 1.7976931348623157e308)) return false;
+    if (!((float)norm < INFINITY)) return false;             // (as it is handed out: the caller sees which steps changed nothing)
     gs = (float)(h.grad_scale * (h.max_norm / fmax(norm, h.max_norm)));
     return true;
 }

@@ -263,7 +263,7 @@ class _AdamWBatch:
     def step(self, t, lr, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=0.0, grad_scale=1.0, max_norm=None, norm=None):
         """One AdamW step, the t-th (t = 1, 2, ...; an int, or an int64 device tensor of one element that a captured step reads when it is
         replayed).  grad_scale multiplies every gradient; max_norm clips their global norm, which goes to `norm` (one fp32 value on the
-        device) — a norm that is not finite leaves everything as it was."""
+        device) — a norm that is not finite there leaves everything as it was."""
         args = native.AdamWArgs(lr, beta1, beta2, eps, weight_decay, grad_scale, 0.0 if max_norm is None else max_norm, 0, 0, self._norm_ptr(norm))
         if max_norm is None and norm is not None:
             raise ValueError("norm is formed with max_norm only (grad_norm forms it alone)")
