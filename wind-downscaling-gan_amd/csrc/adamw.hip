@@ -7,7 +7,7 @@
 // maxima and no other wave needs them.
 //
 // Bound: HBM.  64 M weights with bf16 gradients and copy: 278 us, 6.4 TB/s of exactly the bytes that the formulas name; 128 M with 8-bit
-// states 346 us, 5.9 TB/s, at 90 vector instructions per element (decoding, exact root and quotient, two block maxima, two companding
+// states 345 us, 5.9 TB/s, at 93 vector instructions per element (decoding, exact root and quotient, two block maxima, two companding
 // roots), which alone would take about 300.  The norm of 128 MB of gradients 27 us (4.7 TB/s).  A large copy reaches 5.3 TB/s.
 #include "vec.h"
 #include <algorithm>

@@ -15,7 +15,8 @@
 //
 // Bound: HBM where the tensors are larger than the caches — forward 2, backward 3 times the tensor, which is what the counters show.
 // 16384 x 4096 bf16 forward 48.7 us (5.5 TB/s), backward 76 (5.3, the parameter sums' launch included); 65536 x 1024 fp32 90 and 135 us
-// (5.9 and 6.0 TB/s); 2097152 x 16 fp32 backward 75 us (5.4).  A large copy reaches 5.3 TB/s on the same card.
+// (5.9 and 6.0 TB/s); 2097152 x 16 fp32 backward 75 us (5.6, of which mean and rstd are 0.2).  A large copy reaches 5.3 TB/s on the same
+// card.
 #include "vec.h"
 #include <algorithm>
 
@@ -623,7 +624,8 @@ static LnGeom ln_geom(int64_t P, int64_t C, int type, bool bwd) {
     if (g.K) {
         // Threads per compute unit: a workgroup that stays walks over many rows with its parameters in registers, and each one of the
         // backward writes 8 C bytes of partial sums, so no more of them than keep the memory busy.  Backward, us with 512 / 1024:
-        // 16384 x 4096 bf16 81 / 94, 32768 x 2048 bf16 81 / 95, 262144 x 256 fp32 151 / 156.  Forward, us with 1024 / 2048: 16384 x 4097
+        // 16384 x 4096 bf16 81 / 94, 32768 x 2048 bf16 81 / 95, 262144 x 256 fp32 151 / 156.  (The quotient is cut to a whole number: a
+        // backward workgroup of 320 to 448 threads has its compute unit to itself.)  Forward, us with 1024 / 2048: 16384 x 4097
         // bf16 (320 threads) 65 / 78, 16384 x 5003 fp16 68 / 75; 4194304 x 16 bf16 57 / 57, 32768 x 2048 bf16 51 / 51.
         const int threads = bwd ? 512 : g.NT > 256 ? 1024 : 2048;
         const int64_t rows = (int64_t)(g.L ? g.NT / g.L : 1) * g.U, resident = LN_CUS * std::max(1, threads / g.NT);
@@ -766,7 +768,7 @@ struct LnBwd {
         if (few) {
             // 16 columns per workgroup, more rows at a time, where that still gives few workgroups; us with 16 / 32 columns / in two launches:
             // 256 x 64 fp32 3.3 / 4.1 / 5.2, 512 x 1024 bf16 4.1 / 5.5 / 7.7, 512 x 4096 bf16 8.5 / 6.3 / 16, 256 x 16384 bf16 20 / 14 / 21;
-            // with 1024 rows: 64 columns fp32 6.3 / 10 / 5.3
+            // with 1024 rows: 64 columns fp32 6.3 / 10 / 5.3 (where LN_FEW_ROWS ends; more rows of wide tensors were not measured in one launch)
             const int cols = q.C <= 2048 ? 16 : 32, colblocks = (q.C + cols - 1) / cols, rows = (L ? NT / (L ? L : 1) : 1) * U;
             const int rowblocks = (int)((q.P + rows - 1) / rows);
             hipLaunchKernelGGL((wdg_layernorm_bwd_few_kernel<T, V, K, L, NT, U>), dim3(rowblocks + colblocks), dim3(g.NT), 0, st, q, rowblocks, cols, dgamma, dbeta, accumulate);
