@@ -485,7 +485,7 @@ class HipOps:
             e0, e1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
             torch.cuda.synchronize(self.device)
             with torch.cuda.stream(main):     # (a longer spin ahead of e0 while the host enqueues the rest: what is timed is the streams)
-                torch.cuda._sleep(5 * cycles)
+                torch.cuda._sleep(10 * cycles)
             e0.record(main)
             for st in streams:                # every stream starts behind e0 ... (all waits BEFORE any spin is enqueued)
                 if st is not main:
